@@ -320,6 +320,143 @@ TAE_API int tae_range_info(tae_handle* h, int32_t* n_encoder, int32_t* n_decoder
  * kernels: hi = f16(x * scale) (round to nearest even, denormals kept), lo = f16(x * scale - hi).  Writes n values each. */
 TAE_API int tae_debug_split_f16(const float* x, size_t n, float scale, uint16_t* hi, uint16_t* lo);
 
+/* ---- Sequence operators --------------------------------------------------------------------------------------------------
+ * One layer of a selective state-space sequence model and the reading of its answers, beside the recurrent stacks, the power norm, the
+ * precisions and the error counts above (no reference counterpart).  Forward only, like every entry point here.
+ *  - they need no handle: a call works on the device current in the calling thread, all of its pointers belong to it, and it is ordered by
+ *    `stream` alone; two calls may run at once as long as neither writes what the other reads or writes;
+ *  - activations are TAE_DTYPE_*, the parameters named `float` below fp32; sums, norms, softmax statistics and states are fp32 or wider, and
+ *    every result is rounded once, when it is stored;
+ *  - tensors of activations are (batch, len, channels) with adjacent channels; `*_batch` / `*_row` are the distances, in elements, between
+ *    sequences and between positions, so a slice of a wider tensor needs no copy.  Outputs are contiguous, except norm_residual's residual;
+ *  - `lengths` (device, int32 per sequence; NULL: all of `len`) marks padding: positions at or behind lengths[b] (clamped to 0..len) are not
+ *    read, their outputs are zero, and a final state is the one after the last position in front of them;
+ *  - workspaces belong to the caller (16-byte aligned, tae_*_workspace bytes) and must not be shared by calls that can run at the same time;
+ *  - an empty tensor is refused, except where a length of zero is named. */
+#define TAE_DTYPE_F32 0
+#define TAE_DTYPE_F16 1
+#define TAE_DTYPE_BF16 2
+#define TAE_ACT_SILU 6            /* v * sigmoid(v); sequence operators only */
+
+/* Short causal convolution of each channel: y[t] = act(bias + sum_k weight[k] x[t - taps + 1 + k]); positions in front of the first are
+ * state[0 .. taps-2] (the last inputs of an earlier call, oldest first; NULL: zeros), and state_out receives the last taps-1 inputs seen.
+ * len = 1 is the single-token step.  state_out may be NULL, or be state itself. */
+typedef struct tae_conv_args {
+    int32_t struct_size;          /* = sizeof(tae_conv_args) */
+    int32_t dtype;                /* x, state, y, state_out */
+    int32_t batch, len, channels;
+    int32_t taps;                 /* 1..8 */
+    int32_t act;                  /* TAE_ACT_LINEAR or TAE_ACT_SILU */
+    int32_t reserved;             /* 0 */
+    int64_t x_batch, x_row;
+    const void* x;
+    const float* weight;          /* (channels, taps) */
+    const float* bias;            /* (channels) or NULL */
+    const void* state;            /* (batch, taps - 1, channels) or NULL */
+    const int32_t* lengths;
+    void* y;                      /* (batch, len, channels) */
+    void* state_out;              /* (batch, taps - 1, channels) or NULL */
+} tae_conv_args;
+TAE_API int tae_causal_conv(const tae_conv_args* args, void* stream);
+
+/* Selective state-space scan.  Per channel e and state n, with d = softplus(dt + dt_bias) (or dt + dt_bias with softplus = 0):
+ *     h[t] = exp(d[t] A[e,n]) h[t-1] + d[t] B[t,n] x[t,e],   y[t,e] = (sum_n C[t,n] h[t] + D[e] x[t,e]) * z[t,e] sigmoid(z[t,e])
+ * h starts at `state` (NULL: zeros) and its last value goes to state_out (which may be state itself; required).  Long inputs with few
+ * channels are cut along t and joined again in fixed order: results do not depend on timing.  len = 1 is the single-token step. */
+typedef struct tae_scan_args {
+    int32_t struct_size;          /* = sizeof(tae_scan_args) */
+    int32_t dtype;                /* x, dt, B, C, z, y */
+    int32_t batch, len, channels;
+    int32_t states;               /* 1..64 */
+    int32_t softplus;             /* 1: d = softplus(dt + dt_bias) */
+    int32_t reserved;             /* 0 */
+    int64_t x_batch, x_row, dt_batch, dt_row, b_batch, b_row, c_batch, c_row, z_batch, z_row;
+    const void *x, *dt;           /* (batch, len, channels) */
+    const float* a;               /* (channels, states) */
+    const void *b, *c;            /* (batch, len, states) */
+    const float* d;               /* (channels) or NULL */
+    const void* z;                /* (batch, len, channels) or NULL */
+    const float* dt_bias;         /* (channels) or NULL */
+    const float* state;           /* (batch, channels, states) or NULL */
+    const int32_t* lengths;
+    void* y;
+    float* state_out;             /* (batch, channels, states) */
+    void* workspace;
+    size_t workspace_bytes;
+} tae_scan_args;
+TAE_API size_t tae_selective_scan_workspace(const tae_scan_args* args);      /* reads the sizes and the dtype only; 0: none, or bad sizes */
+TAE_API int tae_selective_scan(const tae_scan_args* args, void* stream);
+
+/* The norms around a block with its gate and residual scale, each row read once:
+ *     p = post ? norm(block) * post_weight + post_bias : block
+ *     r = residual + alpha * scale * gate_act(gate) * p          (block NULL: r = residual)
+ *     normed = norm(r) * pre_weight + pre_bias                   (of r before its rounding)
+ * norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps), mean = 0 with center = 0.  residual_out may be residual itself (same strides). */
+typedef struct tae_norm_args {
+    int32_t struct_size;          /* = sizeof(tae_norm_args) */
+    int32_t dtype;                /* block, gate, normed */
+    int32_t residual_dtype;       /* residual, residual_out: dtype or TAE_DTYPE_F32 */
+    int32_t batch, len, dim;      /* dim 1..32768 */
+    int32_t center;               /* 1: subtract the mean */
+    int32_t gate_act;             /* TAE_ACT_LINEAR, TANH, SIGMOID or SILU */
+    float eps;                    /* > 0 */
+    float alpha;
+    int64_t residual_batch, residual_row, block_batch, block_row;
+    int64_t gate_batch, gate_row; /* gate_row = 0: one gate for each sequence */
+    int64_t out_batch, out_row;   /* residual_out */
+    const void *residual, *block, *gate;
+    const float *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;      /* (dim) or NULL; a bias needs its weight */
+    void* residual_out;           /* NULL only with block NULL */
+    void* normed;                 /* (batch, len, dim), NULL without pre_weight */
+} tae_norm_args;
+TAE_API int tae_norm_residual(const tae_norm_args* args, void* stream);
+
+/* Rows in 8-bit whole numbers with a scale each: scale = max|x| / 127, q = round(127 x / max|x|), halves to even (a row of zeros: all 0).
+ * q rows are q_row bytes apart (a multiple of 16), zero-filled behind cols.  A row with an infinity or NaN has the scale NaN, q 0. */
+TAE_API int tae_quantize_int8(int32_t dtype, const void* x, int64_t x_row, int32_t rows, int32_t cols, int8_t* q, int64_t q_row, float* scale, void* stream);
+
+/* y = (q(x) . weight) * scale(x) * weight_scale + bias: the rows of x are quantised as above inside the call, products are summed in 32-bit
+ * whole numbers (exact), |weight| <= 127.  Weight rows start on 16-byte boundaries, and each, the last one too, can be read up to its next
+ * 16-byte boundary; what stands there does not matter. */
+typedef struct tae_int8_args {
+    int32_t struct_size;          /* = sizeof(tae_int8_args) */
+    int32_t dtype;                /* x, y */
+    int32_t rows, inputs, outputs;/* inputs 1..131072 */
+    int32_t reserved;             /* 0 */
+    int64_t x_row, weight_row;
+    const void* x;                /* (rows, inputs) */
+    const int8_t* weight;         /* (outputs, inputs) */
+    const float* weight_scale;    /* (outputs) */
+    const float* bias;            /* (outputs) or NULL */
+    void* y;                      /* (rows, outputs) */
+    void* workspace;
+    size_t workspace_bytes;
+} tae_int8_args;
+TAE_API size_t tae_int8_linear_workspace(const tae_int8_args* args);
+TAE_API int tae_int8_linear(const tae_int8_args* args, void* stream);
+
+/* Reading a model's answers: for each row of logits the log probability of the given token, the entropy (nats) and the `top` most probable
+ * tokens, equal ones in ascending order.  A logit of -inf is a token that cannot occur; in a row of nothing else every log probability is
+ * -inf, the entropy 0.  A row with +inf or NaN has none: NaN, ids -1.  A negative token marks a row without one (log probability 0, as for
+ * padding), one at or above vocab gives NaN.  logits rows are logits_row elements apart. */
+typedef struct tae_logprobs_args {
+    int32_t struct_size;          /* = sizeof(tae_logprobs_args) */
+    int32_t dtype;                /* logits */
+    int32_t token_bytes;          /* 4 or 8: int32 or int64 tokens */
+    int32_t rows, vocab;
+    int32_t top;                  /* 0..32, at most vocab */
+    int64_t logits_row;
+    const void* logits;           /* (rows, vocab) */
+    const void* tokens;           /* (rows) */
+    float *logp, *entropy;        /* (rows) */
+    int64_t* top_ids;             /* (rows, top); NULL with top = 0 */
+    float* top_logp;
+    void* workspace;
+    size_t workspace_bytes;
+} tae_logprobs_args;
+TAE_API size_t tae_token_logprobs_workspace(const tae_logprobs_args* args);
+TAE_API int tae_token_logprobs(const tae_logprobs_args* args, void* stream);
+
 TAE_API const char* tae_last_error(void);
 TAE_API int tae_abi_version(void);
 

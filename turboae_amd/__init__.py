@@ -8,7 +8,7 @@ from .config import TurboAEConfig
 from .interleaver import rand_interleaver
 from . import weights, philox
 
-__all__ = ["TurboAEConfig", "rand_interleaver", "weights", "philox", "Channel_AE_HIP"]
+__all__ = ["TurboAEConfig", "rand_interleaver", "weights", "philox", "Channel_AE_HIP", "sequence"]
 
 
 def __getattr__(name):
@@ -16,4 +16,7 @@ def __getattr__(name):
     if name == "Channel_AE_HIP":
         from .channel_ae import Channel_AE_HIP
         return Channel_AE_HIP
+    if name == "sequence":
+        from importlib import import_module
+        return import_module(".sequence", __name__)
     raise AttributeError(name)

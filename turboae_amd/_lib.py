@@ -35,6 +35,26 @@ class TaeNoiseOpts(C.Structure):
                 ("radar_power", C.c_float), ("p_gg", C.c_float), ("p_bb", C.c_float)]
 
 
+def _struct(name: str, **kinds: str) -> type:
+    """A ctypes structure from `kind="field field ..."` groups in the header's order (struct_size first)."""
+    types = {"i32": C.c_int32, "i64": C.c_int64, "f32": C.c_float, "ptr": C.c_void_p, "size": C.c_size_t}
+    return type(name, (C.Structure,), {"_fields_": [(f, types[k.split("_")[0]]) for k, names in kinds.items() for f in names.split()]})
+
+
+# arguments of the sequence operators (include/turboae_hip.h); every structure starts with struct_size
+TaeConvArgs = _struct("TaeConvArgs", i32="struct_size dtype batch len channels taps act reserved", i64="x_batch x_row",
+                      ptr="x weight bias state lengths y state_out")
+TaeScanArgs = _struct("TaeScanArgs", i32="struct_size dtype batch len channels states softplus reserved",
+                      i64="x_batch x_row dt_batch dt_row b_batch b_row c_batch c_row z_batch z_row",
+                      ptr="x dt a b c d z dt_bias state lengths y state_out workspace", size="workspace_bytes")
+TaeNormArgs = _struct("TaeNormArgs", i32="struct_size dtype residual_dtype batch len dim center gate_act", f32="eps alpha",
+                      i64="residual_batch residual_row block_batch block_row gate_batch gate_row out_batch out_row",
+                      ptr="residual block gate scale post_weight post_bias pre_weight pre_bias residual_out normed")
+TaeInt8Args = _struct("TaeInt8Args", i32="struct_size dtype rows inputs outputs reserved", i64="x_row weight_row",
+                      ptr="x weight weight_scale bias y workspace", size="workspace_bytes")
+TaeLogprobsArgs = _struct("TaeLogprobsArgs", i32="struct_size dtype token_bytes rows vocab top", i64="logits_row",
+                          ptr="logits tokens logp entropy top_ids top_logp workspace", size="workspace_bytes")
+
 RANGE_HIGH, RANGE_LOW, RANGE_FELL_BACK = 1, 2, 4        # TAE_RANGE_* bits of tae_range_status
 
 NOISE_KIND = {"awgn": 0, "t-dist": 1, "radar": 2, "ge_awgn": 3, "bec": 4, "bsc": 5, "ge": 6, "fading": 7}      # TAE_NOISE_*
@@ -69,6 +89,15 @@ SIGNATURES = {
     "tae_range_status": (C.c_int, [_P, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "tae_calibrate_range": (C.c_int, [_P, _P, _P, C.c_int32]),
     "tae_range_info": (C.c_int, [_P, C.POINTER(C.c_int32), C.POINTER(C.c_int32), _P, C.c_int32, C.POINTER(C.c_int32)]),
+    "tae_causal_conv": (C.c_int, [C.POINTER(TaeConvArgs), _P]),
+    "tae_selective_scan_workspace": (C.c_size_t, [C.POINTER(TaeScanArgs)]),
+    "tae_selective_scan": (C.c_int, [C.POINTER(TaeScanArgs), _P]),
+    "tae_norm_residual": (C.c_int, [C.POINTER(TaeNormArgs), _P]),
+    "tae_quantize_int8": (C.c_int, [C.c_int32, _P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P]),
+    "tae_int8_linear_workspace": (C.c_size_t, [C.POINTER(TaeInt8Args)]),
+    "tae_int8_linear": (C.c_int, [C.POINTER(TaeInt8Args), _P]),
+    "tae_token_logprobs_workspace": (C.c_size_t, [C.POINTER(TaeLogprobsArgs)]),
+    "tae_token_logprobs": (C.c_int, [C.POINTER(TaeLogprobsArgs), _P]),
     "tae_debug_split_f16": (C.c_int, [_P, C.c_size_t, C.c_float, _P, _P]),
 }
 

@@ -1,0 +1,96 @@
+// What the sequence operators (turboae_seq_*.hip) share: element types, vector loads and stores, reductions over lanes, and the checks of
+// their C entry points.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <exception>
+
+#include "../../include/turboae_hip.h"
+
+namespace tae {
+
+int fail_msg(int code, const char* msg);      // sets the calling thread's tae_last_error string, returns `code`
+
+namespace seq {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+// V adjacent elements; loads and stores of up to 16 bytes are one instruction each
+template <class T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+    T v[V];
+};
+
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+template <class T, int V>
+__device__ __forceinline__ void store(T* p, const Pack<T, V>& a) { *reinterpret_cast<Pack<T, V>*>(p) = a; }
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }       // relative error 2^-22 |x| and up to one ulp
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
+// v * sigmoid(v); at -inf the product would be -inf * 0
+__device__ __forceinline__ float silu(float x) { return x < -100.0f ? 0.0f * (x == x ? 1.0f : x) : x * sigmoid(x); }
+// log(1 + e^x).  With u = 1 + e rounded, log(u) e / (u - 1) has the relative accuracy that log(u) alone loses for small e (the rounding of u
+// moves log(u) and u - 1 by the same factor to first order).
+__device__ __forceinline__ float softplus(float x) {
+    if (x > 20.0f) return x;
+    const float e = exp_fast(x), u = 1.0f + e, m = u - 1.0f;
+    return m == 0.0f ? e : __builtin_amdgcn_logf(u) * kLn2 * (e / m);
+}
+
+// sums and maxima over the 2^k adjacent lanes that share a value (W a power of two up to 64)
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+template <int W>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+inline size_t dtype_bytes(int32_t t) { return t == TAE_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_ok(int32_t t) { return t >= TAE_DTYPE_F32 && t <= TAE_DTYPE_BF16; }
+inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Largest V of {16 / size, 4 / size, 1} that divides every given size and stride and to which every pointer is aligned.
+struct Width {
+    size_t bytes;
+    int64_t all = 0;                             // bits of every size, stride (in elements) and address
+    explicit Width(size_t element) : bytes(element) {}
+    Width& elements(int64_t n) { all |= n * (int64_t)bytes; return *this; }
+    Width& pointer(const void* p) { all |= (int64_t)reinterpret_cast<uintptr_t>(p); return *this; }
+    bool fits(size_t n) const { return (all & (int64_t)(n - 1)) == 0; }
+};
+
+// A launch of n workgroups, n up to 2^40: one grid dimension holds fewer than 2^32 work items.  Workgroups behind the last have nothing to do.
+constexpr int kGridX = 1 << 20;
+inline dim3 grid_of(int64_t n) { return n <= kGridX ? dim3((uint32_t)n) : dim3(kGridX, (uint32_t)ceil_div(n, kGridX)); }
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
+
+// The launches of a C entry point: no exception leaves it, and a failed launch is an error of this call.
+template <class F>
+int guarded(F&& f) {
+    try {
+        const int rc = f();
+        if (rc != TAE_OK) return rc;
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? TAE_OK : fail_msg(TAE_EHIP, hipGetErrorString(e));
+    } catch (const std::exception& e) {
+        return fail_msg(TAE_ENOMEM, e.what());
+    } catch (...) {
+        return fail_msg(TAE_ENOMEM, "unknown exception");
+    }
+}
+
+}  // namespace seq
+}  // namespace tae

@@ -1,0 +1,248 @@
+// tae_norm_residual: the norms before and after a block fused with its gate and residual scale.
+//
+//     p = post ? norm(block) w + b : block,   r = residual + alpha scale act(gate) p,   normed = norm(r) w' + b'
+//
+// Bound by memory: a row is read once and stays in registers (T lanes hold V adjacent elements in each of NV steps); mean and variance are
+// two sums over those registers, the second of the squares of what is left of the first, so that a large mean costs no digits.
+#include "turboae_seq.hpp"
+
+namespace tae {
+namespace seq {
+
+struct NormArgs {
+    const void *residual, *block, *gate;
+    const float *scale, *post_w, *post_b, *pre_w, *pre_b;
+    void *out, *normed;
+    int64_t rs_b, rs_r, bl_b, bl_r, ga_b, ga_r, ou_b, ou_r;
+    int rows, len, dim, center, gate_act;
+    float eps, alpha;
+};
+
+__device__ __forceinline__ float gate_value(float g, int act) {
+    switch (act) {
+        case TAE_ACT_TANH: return 2.0f * sigmoid(2.0f * g) - 1.0f;
+        case TAE_ACT_SIGMOID: return sigmoid(g);
+        case TAE_ACT_SILU: return silu(g);
+        default: return g;
+    }
+}
+
+// Sum over the TPR lanes of a row; every lane gets it.
+template <int TPR, int THREADS>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+    v = lanes_sum<(TPR < 64 ? TPR : 64)>(v);
+    if constexpr (TPR > 64) {
+        const int w = threadIdx.x >> 6;
+        __syncthreads();                        // the last sum has been read
+        if ((threadIdx.x & 63) == 0) lds[w] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v += lds[i];
+    }
+    return v;
+}
+
+template <class T, class R, int V, int NV, int TPR, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
+    __shared__ float lds[16];
+    const int lane = threadIdx.x % TPR;
+    const int64_t row = block_index() * (THREADS / TPR) + threadIdx.x / TPR;
+    if (row >= a.rows) return;                  // whole workgroups, or with TPR = 64 whole waves, which meet no barrier
+    const int64_t b = row / a.len, t = row % a.len;
+    const R* rs = (const R*)a.residual + b * a.rs_b + t * a.rs_r;
+    const float inv = 1.0f / (float)a.dim;
+    float r[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int e = (j * TPR + lane) * V;
+        if (e < a.dim) {
+            const Pack<R, V> x = load<R, V>(rs + e);
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[j][i] = (float)x.v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[j][i] = 0.0f;
+        }
+    }
+    auto norm_of = [&](const float (&v)[NV][V], float& mean, float& rstd) {
+        mean = 0.0f;
+        float s = 0.0f;
+        if (a.center) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) s += v[j][i];
+            mean = row_sum<TPR, THREADS>(s, lds) * inv;
+            s = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const bool in = (j * TPR + lane) * V < a.dim;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = in ? v[j][i] - mean : 0.0f;
+                s = __builtin_fmaf(d, d, s);
+            }
+        }
+        rstd = 1.0f / sqrtf(row_sum<TPR, THREADS>(s, lds) * inv + a.eps);
+    };
+    if (a.block) {
+        const T* bl = (const T*)a.block + b * a.bl_b + t * a.bl_r;
+        const T* ga = a.gate ? (const T*)a.gate + b * a.ga_b + t * a.ga_r : nullptr;
+        float p[NV][V];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * TPR + lane) * V;
+            if (e < a.dim) {
+                const Pack<T, V> x = load<T, V>(bl + e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) p[j][i] = (float)x.v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) p[j][i] = 0.0f;
+            }
+        }
+        float mean = 0.0f, rstd = 1.0f;
+        if (a.post_w) norm_of(p, mean, rstd);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * TPR + lane) * V;
+            if (e >= a.dim) continue;
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = p[j][i];
+            if (a.post_w) {
+                const Pack<float, V> w = load<float, V>(a.post_w + e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] = (f[i] - mean) * rstd * w.v[i];
+                if (a.post_b) {
+                    const Pack<float, V> c = load<float, V>(a.post_b + e);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f[i] += c.v[i];
+                }
+            }
+            if (a.scale) {
+                const Pack<float, V> w = load<float, V>(a.scale + e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] *= w.v[i];
+            }
+            if (ga) {
+                const Pack<T, V> g = load<T, V>(ga + e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] *= gate_value((float)g.v[i], a.gate_act);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[j][i] = __builtin_fmaf(a.alpha, f[i], r[j][i]);
+        }
+    }
+    if (a.out) {
+        R* o = (R*)a.out + b * a.ou_b + t * a.ou_r;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * TPR + lane) * V;
+            if (e >= a.dim) continue;
+            Pack<R, V> x;
+#pragma unroll
+            for (int i = 0; i < V; ++i) x.v[i] = (R)r[j][i];
+            store<R, V>(o + e, x);
+        }
+    }
+    if (a.normed) {
+        float mean, rstd;
+        norm_of(r, mean, rstd);
+        T* o = (T*)a.normed + row * a.dim;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * TPR + lane) * V;
+            if (e >= a.dim) continue;
+            const Pack<float, V> w = load<float, V>(a.pre_w + e);
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = (r[j][i] - mean) * rstd * w.v[i];
+            if (a.pre_b) {
+                const Pack<float, V> c = load<float, V>(a.pre_b + e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] += c.v[i];
+            }
+            Pack<T, V> x;
+#pragma unroll
+            for (int i = 0; i < V; ++i) x.v[i] = (T)f[i];
+            store<T, V>(o + e, x);
+        }
+    }
+}
+
+template <class T, class R, int V, int NV, int TPR, int THREADS>
+static void launch_norm_as(const NormArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((norm_residual_kernel<T, R, V, NV, TPR, THREADS>), grid_of(ceil_div(a.rows, THREADS / TPR)), dim3(THREADS), 0, st, a);
+}
+
+// Lanes and steps that hold a row: one wave for short rows, else as many lanes as leave each at most 32 elements.
+template <class T, class R, int V>
+static void launch_norm_width(const NormArgs& a, hipStream_t st) {
+    const int vecs = (int)ceil_div(a.dim, V);
+    constexpr int M = 8 / V;                    // steps of V that are one step of 8
+    if (vecs <= 64 * M) launch_norm_as<T, R, V, M, 64, 256>(a, st);
+    else if (vecs <= 128 * M) launch_norm_as<T, R, V, 2 * M, 64, 256>(a, st);
+    else if (vecs <= 256 * M) launch_norm_as<T, R, V, M, 256, 256>(a, st);
+    else if (vecs <= 512 * M) launch_norm_as<T, R, V, 2 * M, 256, 256>(a, st);
+    else if (vecs <= 1024 * M) launch_norm_as<T, R, V, 4 * M, 256, 256>(a, st);
+    else if (vecs <= 2048 * M) launch_norm_as<T, R, V, 2 * M, 1024, 1024>(a, st);
+    else launch_norm_as<T, R, V, 4 * M, 1024, 1024>(a, st);
+}
+
+template <class T, class R>
+static void launch_norm(const NormArgs& a, int width, hipStream_t st) {
+    if (width == 8) launch_norm_width<T, R, 8>(a, st);
+    else if (width == 4) launch_norm_width<T, R, 4>(a, st);
+    else launch_norm_width<T, R, 1>(a, st);
+}
+
+}  // namespace seq
+}  // namespace tae
+
+extern "C" int tae_norm_residual(const tae_norm_args* p, void* stream) {
+    using namespace tae;
+    using namespace tae::seq;
+    if (!p || p->struct_size != (int32_t)sizeof(tae_norm_args)) return fail_msg(TAE_EINVAL, "tae_norm_args: NULL or struct_size mismatch (ABI)");
+    if (!dtype_ok(p->dtype)) return fail_msg(TAE_EINVAL, "norm_residual: dtype must be a TAE_DTYPE_* code");
+    if (p->residual_dtype != p->dtype && p->residual_dtype != TAE_DTYPE_F32) return fail_msg(TAE_EINVAL, "norm_residual: the residual has the block's type or fp32");
+    if (p->batch < 1 || p->len < 1 || (int64_t)p->batch * p->len > INT32_MAX) return fail_msg(TAE_EINVAL, "norm_residual: batch and len must be >= 1, their product below 2^31");
+    if (p->dim < 1 || p->dim > 32768) return fail_msg(TAE_EINVAL, "norm_residual: dim must be in 1..32768");
+    if (!(p->eps > 0.0f)) return fail_msg(TAE_EINVAL, "norm_residual: eps must be > 0");
+    if (p->gate_act != TAE_ACT_LINEAR && p->gate_act != TAE_ACT_TANH && p->gate_act != TAE_ACT_SIGMOID && p->gate_act != TAE_ACT_SILU)
+        return fail_msg(TAE_EINVAL, "norm_residual: gate_act must be linear, tanh, sigmoid or silu");
+    if (!p->residual) return fail_msg(TAE_EINVAL, "norm_residual: residual is NULL");
+    if (p->block && !p->residual_out) return fail_msg(TAE_EINVAL, "norm_residual: a block needs residual_out");
+    if (!p->block && (p->gate || p->scale || p->post_weight)) return fail_msg(TAE_EINVAL, "norm_residual: gate, scale and post_weight need a block");
+    if ((p->post_bias && !p->post_weight) || (p->pre_bias && !p->pre_weight)) return fail_msg(TAE_EINVAL, "norm_residual: a bias needs its weight");
+    if ((p->normed != nullptr) != (p->pre_weight != nullptr)) return fail_msg(TAE_EINVAL, "norm_residual: normed and pre_weight come together");
+    if (!p->residual_out && !p->normed) return fail_msg(TAE_EINVAL, "norm_residual: nothing to write");
+    if (p->residual_out == p->residual && p->residual && (p->out_batch != p->residual_batch || p->out_row != p->residual_row))
+        return fail_msg(TAE_EINVAL, "norm_residual: an in-place residual_out has the residual's strides");
+    const size_t tb = dtype_bytes(p->dtype), rb = dtype_bytes(p->residual_dtype);
+    Width wt(tb), wr(rb), wf(4);
+    wt.elements(p->dim).pointer(p->normed);
+    if (p->block) wt.pointer(p->block).elements(p->block_batch).elements(p->block_row);
+    if (p->gate) wt.pointer(p->gate).elements(p->gate_batch).elements(p->gate_row);
+    wr.elements(p->dim).pointer(p->residual).elements(p->residual_batch).elements(p->residual_row);
+    if (p->residual_out) wr.pointer(p->residual_out).elements(p->out_batch).elements(p->out_row);
+    wf.elements(p->dim).pointer(p->scale).pointer(p->post_weight).pointer(p->post_bias).pointer(p->pre_weight).pointer(p->pre_bias);
+    int width = 1;
+    for (int v : {8, 4})
+        if (width == 1 && p->dim % v == 0 && wt.fits(v * tb < 16 ? v * tb : 16) && wr.fits(v * rb < 16 ? v * rb : 16) && wf.fits(16)) width = v;
+    NormArgs a{p->residual, p->block, p->gate, p->scale, p->post_weight, p->post_bias, p->pre_weight, p->pre_bias, p->residual_out, p->normed,
+               p->residual_batch, p->residual_row, p->block_batch, p->block_row, p->gate_batch, p->gate_row, p->out_batch, p->out_row,
+               p->batch * p->len, p->len, p->dim, p->center ? 1 : 0, p->gate_act, p->eps, p->alpha};
+    return guarded([&] {
+        hipStream_t st = (hipStream_t)stream;
+        const bool same = p->residual_dtype == p->dtype;
+        switch (p->dtype) {
+            case TAE_DTYPE_F32: launch_norm<float, float>(a, width, st); break;
+            case TAE_DTYPE_F16: same ? launch_norm<f16, f16>(a, width, st) : launch_norm<f16, float>(a, width, st); break;
+            default: same ? launch_norm<bf16, bf16>(a, width, st) : launch_norm<bf16, float>(a, width, st); break;
+        }
+        return (int)TAE_OK;
+    });
+}
