@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <exception>
 
 #include "../../include/turboae_hip.h"
@@ -33,14 +34,12 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }       // relative error 2^-22 |x| and up to one ulp
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
-// v * sigmoid(v); at -inf the product would be -inf * 0
-__device__ __forceinline__ float silu(float x) { return x < -100.0f ? 0.0f * (x == x ? 1.0f : x) : x * sigmoid(x); }
-// log(1 + e^x).  With u = 1 + e rounded, log(u) e / (u - 1) has the relative accuracy that log(u) alone loses for small e (the rounding of u
-// moves log(u) and u - 1 by the same factor to first order).
+__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+// log(1 + e^x) = max(x, 0) + log(1 + w), w = e^-|x|.  u = 1 + w loses the last digits of a small w; log(u) plus what was lost, w - (u - 1), has
+// the relative accuracy that log(u) alone has not (next to u = 1 the two differ by the loss itself).
 __device__ __forceinline__ float softplus(float x) {
-    if (x > 20.0f) return x;
-    const float e = exp_fast(x), u = 1.0f + e, m = u - 1.0f;
-    return m == 0.0f ? e : __builtin_amdgcn_logf(u) * kLn2 * (e / m);
+    const float w = exp_fast(-fabsf(x)), u = 1.0f + w;
+    return fmaxf(x, 0.0f) + __builtin_fmaf(__builtin_amdgcn_logf(u), kLn2, w - (u - 1.0f));
 }
 
 // sums and maxima over the 2^k adjacent lanes that share a value (W a power of two up to 64)

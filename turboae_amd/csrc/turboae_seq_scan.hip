@@ -10,21 +10,78 @@ struct ScanArgs {
     const int32_t* lengths;
     void* y;
     float* state_out;
-    float *steps, *states;                       // workspace: (batch, pieces, channels) sums of d; (batch, pieces + 1, channels, states)
+    float *steps, *states;                       // workspace: (batch, pieces, channels) sums of d; (batch, pieces + 1, states, channels)
     int64_t x_b, x_r, dt_b, dt_r, b_b, b_r, c_b, c_r, z_b, z_r;
-    int len, channels, n, softplus, groups, pieces, piece_len;      // groups of CW channels; pieces of piece_len positions
+    int len, channels, n, softplus, gate, groups, pieces, piece_len;      // groups of CW channels; pieces of piece_len positions
     int64_t blocks;
 };
 
 constexpr int kScanThreads = 256;
-constexpr int kTile = 32;                        // positions staged in LDS at once
 
-// P adjacent lanes share a channel, each holds S of its states.  ENDS: only the state behind a piece, started from zero (the first piece: from
-// `state`), and the sum of its steps, whose exponential carries a state across the piece.
-template <class T, int S, int P, bool ENDS>
+// Elements of a row as they were loaded, in whole registers and taken out only when they are used, so that a load stays in flight until
+// then.  V = 4: four adjacent ones, one load; V = 1: four, a load each; V = 0: one.  Elements behind the row repeat its last ones.
+template <class T, int V>
+struct Loaded {
+    uint32_t w[V == 4 ? sizeof(T) : V == 1 ? 4 : 1];
+    __device__ __forceinline__ static uint32_t one(const T* p) {
+        if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(p);
+        else return *reinterpret_cast<const uint16_t*>(p);
+    }
+    __device__ __forceinline__ void from(const T* row, int at, int width) {
+        if constexpr (V == 4 && sizeof(T) == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(row + min(at, width - 4));
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else if constexpr (V == 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(row + min(at, width - 4));
+            w[0] = u.x, w[1] = u.y;
+        } else if constexpr (V == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = one(row + min(at + i, width - 1));
+        } else {
+            w[0] = one(row + min(at, width - 1));
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[i]);
+        } else {
+            const uint32_t u = V != 4 ? w[i] : i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
+            return (float)__builtin_bit_cast(T, (uint16_t)u);
+        }
+    }
+};
+
+// Sum over the P adjacent lanes of a channel for four positions at once.  Lanes that hold the same sum twice are put to use: in P = 16 the
+// first exchange leaves positions 0 | 1 (2 | 3) in the two halves of a row and the second 0, 2, 1, 3 in its four quads - 11 instructions
+// instead of 16.  The position whose sum a lane ends up with is `reduced_position`.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_choose(bool second, float v0, float v1) {
+    const float a = dpp_add<CTRL>(v0), b = dpp_add<CTRL>(v1);      // by all lanes, before the choice
+    return second ? b : a;
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128;      // quad_perm [1,0,3,2], [2,3,0,1]; row_half_mirror; row_ror:8
+
+template <int P>
+__device__ __forceinline__ int reduced_position(int lane) {
+    if constexpr (P == 16) return ((lane >> 3) & 1) | ((lane >> 1) & 2);
+    return (lane >> 2) & 1;                     // P = 8: pairs 0 | 1 and 2 | 3
+}
+
+// P lanes share a channel, each holds S of its states (n = s P + p).  A workgroup takes 256 / P channels and walks the positions of its
+// piece in tiles of TT: steps d and d x (once for each channel and position), B and C go through LDS as rows over the positions, so that a
+// lane reads four positions with one 16-byte load; two buffers, one barrier for each tile; the next tile's loads are in flight meanwhile.
+// ENDS: only the state behind a piece, started from zero (the first piece: from `state`), and the sum of its steps, whose exponential
+// carries a state across the piece.  V: 4 where rows allow loads of four channels and four states, else 1.
+template <class T, int S, int P, int TT, int V, bool ENDS>
 __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q) {
-    constexpr int CW = kScanThreads / P, N = S * P, DS = kTile + 4;
-    __shared__ float sd[CW * DS], sx[CW * DS], sb[kTile * N], sc[ENDS ? 1 : kTile * N];
+    constexpr int CW = kScanThreads / P, N = S * P, DS = TT + 4;
+    constexpr int R = TT * CW / 4 / kScanThreads, RB = (TT * N + kScanThreads - 1) / kScanThreads;      // groups of four, elements for each thread
+    static_assert(R >= 1 && TT * CW % (4 * kScanThreads) == 0, "a tile is whole groups of four for every thread");
+    __shared__ float sd[2][CW * DS], sx[2][CW * DS], sb[2][N * DS], sc[ENDS ? 1 : 2][ENDS ? 4 : N * DS], sy[ENDS ? 1 : 2][ENDS ? 4 : CW * DS];
     int64_t id = block_index();
     if (id >= q.blocks) return;
     const int group = (int)(id % q.groups);
@@ -40,149 +97,624 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
     float a2[S], h[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int k = p * S + s;
+        const int k = s * P + p;
         a2[s] = mine && k < q.n ? q.a[(int64_t)e * q.n + k] * kLog2e : 0.0f;
         h[s] = 0.0f;
     }
-    float* kept = q.pieces > 1 ? q.states + ((b * (q.pieces + 1)) * E + e) * q.n : nullptr;     // [0]: the start, [k + 1]: behind piece k
-    const int64_t kept_step = (int64_t)E * q.n;
-    if (mine && piece == 0 && q.state && (ENDS || q.pieces == 1)) {
+    if (mine && (ENDS || q.pieces == 1) && piece == 0 && q.state) {
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (p * S + s < q.n) h[s] = q.state[(b * E + e) * q.n + p * S + s];
+            if (s * P + p < q.n) h[s] = q.state[(b * E + e) * q.n + s * P + p];
     }
-    if (ENDS && mine && piece == 0) {            // the start is kept: state_out may be the state
+    if (!ENDS && mine && q.pieces > 1) {
+        const float* kept = q.states + (b * (q.pieces + 1) + piece) * q.n * (int64_t)E + e;
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (p * S + s < q.n) kept[p * S + s] = h[s];
-    }
-    if (!ENDS && q.pieces > 1 && mine && (stop > begin || piece == last_piece)) {
-        if (piece == 0) {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (p * S + s < q.n) h[s] = kept[p * S + s];
-        }
-        for (int k = 0; k < piece; ++k) {
-            const float sum = q.steps[(b * q.pieces + k) * E + e];
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (p * S + s < q.n) h[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(sum * a2[s]), h[s], kept[(k + 1) * kept_step + p * S + s]);
-        }
+            if (s * P + p < q.n) h[s] = kept[(int64_t)(s * P + p) * E];
     }
     float sum = 0.0f;
     const T* x = (const T*)q.x + b * q.x_b;
     const T* dt = (const T*)q.dt + b * q.dt_b;
     const T* bm = (const T*)q.b + b * q.b_b;
     const T* cm = (const T*)q.c + b * q.c_b;
-    const T* z = q.z ? (const T*)q.z + b * q.z_b : nullptr;
+    const T* z = (const T*)q.z + b * q.z_b;          // without a gate: x again, unused
     T* y = (T*)q.y + b * q.len * (int64_t)E;
-    for (int t0 = begin; t0 < (ENDS ? stop : end); t0 += kTile) {
-        __syncthreads();
-        if (t0 < stop) {
-            for (int i = tid; i < kTile * CW; i += kScanThreads) {
-                const int t = i / CW, c = i % CW;
-                float d = 0.0f, dx = 0.0f;
-                if (t0 + t < stop && e0 + c < E) {
-                    d = (float)dt[(t0 + t) * q.dt_r + e0 + c] + (q.dt_bias ? q.dt_bias[e0 + c] : 0.0f);
-                    if (q.softplus) d = softplus(d);
-                    dx = d * (float)x[(t0 + t) * q.x_r + e0 + c];
-                }
-                sd[c * DS + t] = d;
-                sx[c * DS + t] = dx;
+
+    using Raw4 = Loaded<T, V>;
+    using Raw1 = Loaded<T, 0>;
+    constexpr int CQ = CW / 4;
+    float bias[4];                               // of this thread's channels: the same four in every group, because CQ divides 256
+    const int cq = (tid % CQ) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = q.dt_bias && e0 + cq + i < E ? q.dt_bias[e0 + cq + i] : 0.0f;
+    float dcoef[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dcoef[i] = !ENDS && q.d && e0 + cq + i < E ? q.d[e0 + cq + i] : 0.0f;
+    // Where this thread's groups of four lie in a tile: rows at or behind `rows` repeat the last one in front of it, as elements behind a row
+    // repeat its last ones, so that every load is unconditional and stays in flight until `stage` uses it.
+    struct Offsets {
+        int64_t x[R], dt[R], z[R], b[RB], c[RB];
+    };
+    auto offsets = [&](int rows) {
+        Offsets o;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int64_t t = min((j * kScanThreads + tid) / CQ, rows - 1);
+            o.x[j] = t * q.x_r;
+            o.dt[j] = t * q.dt_r;
+            o.z[j] = t * q.z_r;
+        }
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            const int64_t t = min((j * kScanThreads + tid) / N, rows - 1);
+            o.b[j] = t * q.b_r;
+            o.c[j] = t * q.c_r;
+        }
+        return o;
+    };
+    struct Raw {
+        Raw4 x[R], dt[R], z[R];
+        Raw1 b[RB], c[RB];
+    };
+    Offsets off;
+    auto fetch = [&](Raw& r, int t0) {
+        if (t0 + TT > stop) off = offsets(stop - t0);        // the last one
+        const int64_t t = t0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            r.x[j].from(x + t * q.x_r + off.x[j], e0 + cq, E);
+            r.dt[j].from(dt + t * q.dt_r + off.dt[j], e0 + cq, E);
+            if constexpr (!ENDS) r.z[j].from(z + t * q.z_r + off.z[j], e0 + cq, E);
+        }
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            const int k = (j * kScanThreads + tid) % N;
+            r.b[j].from(bm + t * q.b_r + off.b[j], k, q.n);
+            if constexpr (!ENDS) r.c[j].from(cm + t * q.c_r + off.c[j], k, q.n);
+        }
+    };
+    // positions at or behind `stop` get step 0: they keep the state.  What was repeated is replaced, not multiplied by 0: it may be infinite
+    auto stage = [&](const Raw& r, int t0, int buf) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int t = (j * kScanThreads + tid) / CQ;
+            const bool in = t0 + t < stop;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float d = r.dt[j][i] + bias[i];
+                if (q.softplus) d = softplus(d);
+                const float dx = d * r.x[j][i];
+                sd[buf][(cq + i) * DS + t] = in ? d : 0.0f;
+                sx[buf][(cq + i) * DS + t] = in ? dx : 0.0f;
             }
-            for (int i = tid; i < kTile * N; i += kScanThreads) {
-                const int t = i / N, k = i % N;
+        }
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            const int i = j * kScanThreads + tid, t = i / N, k = i % N;
+            if (TT * N % kScanThreads == 0 || i < TT * N) {
                 const bool in = t0 + t < stop && k < q.n;
-                sb[i] = in ? (float)bm[(t0 + t) * q.b_r + k] : 0.0f;
-                if constexpr (!ENDS) sc[i] = in ? (float)cm[(t0 + t) * q.c_r + k] : 0.0f;
+                sb[buf][k * DS + t] = in ? r.b[j][0] : 0.0f;
+                if constexpr (!ENDS) sc[buf][k * DS + t] = in ? r.c[j][0] : 0.0f;
             }
-            __syncthreads();
-            // positions behind `stop` have step 0: they keep the state
-            for (int t = 0; t < kTile; t += 4) {
-                const Pack<float, 4> d4 = load<float, 4>(&sd[ch * DS + t]), x4 = load<float, 4>(&sx[ch * DS + t]);
+        }
+    };
+    const int first = begin, behind = ENDS ? stop : end;
+    Raw now, next;
+    int tile = 0;
+    // what the loop uses has arrived before it: a wait inside would wait for the loads in flight too
+#pragma unroll
+    for (int s = 0; s < S; ++s) asm volatile("" : "+v"(h[s]), "+v"(a2[s]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(bias[i]), "+v"(dcoef[i]));
+    if (first < stop) {
+        off = offsets(TT);
+        fetch(now, first);
+        stage(now, first, 0);
+        __syncthreads();
+    }
+    for (int t0 = first; t0 < behind; t0 += TT, ++tile) {
+        const int buf = tile & 1;
+        const bool more = t0 + TT < stop;
+        if (more) fetch(next, t0 + TT);
+        if (t0 < stop) {
+            const float* pd = &sd[buf][ch * DS];
+            const float* px = &sx[buf][ch * DS];
+            Pack<float, 4> d4 = load<float, 4>(pd), x4 = load<float, 4>(px), b4[S], c4[S];
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                b4[s] = load<float, 4>(&sb[buf][(s * P + p) * DS]);
+                if constexpr (!ENDS) c4[s] = load<float, 4>(&sc[buf][(s * P + p) * DS]);
+            }
+#pragma unroll 4
+            for (int t = 0; t < TT; t += 4) {
+                // the next four positions' operands are read while these are worked on (at the last, four floats of padding)
+                const Pack<float, 4> dn = load<float, 4>(pd + t + 4), xn = load<float, 4>(px + t + 4);
+                Pack<float, 4> bn[S], cn[S];
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    bn[s] = load<float, 4>(&sb[buf][(s * P + p) * DS + t + 4]);
+                    if constexpr (!ENDS) cn[s] = load<float, 4>(&sc[buf][(s * P + p) * DS + t + 4]);
+                }
                 float out[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float o = 0.0f;
+                for (int s = 0; s < S; ++s)
 #pragma unroll
-                    for (int s = 0; s < S; ++s) {
+                    for (int i = 0; i < 4; ++i) {
                         const float g = __builtin_amdgcn_exp2f(d4.v[i] * a2[s]);
-                        h[s] = __builtin_fmaf(g, h[s], x4.v[i] * sb[(t + i) * N + p * S + s]);
-                        if constexpr (!ENDS) o = __builtin_fmaf(h[s], sc[(t + i) * N + p * S + s], o);
+                        h[s] = __builtin_fmaf(g, h[s], x4.v[i] * b4[s].v[i]);
+                        if constexpr (!ENDS) out[i] = s == 0 ? h[s] * c4[s].v[i] : __builtin_fmaf(h[s], c4[s].v[i], out[i]);
                     }
-                    if constexpr (ENDS) sum += d4.v[i];
-                    else out[i] = lanes_sum<P>(o);
+                if constexpr (ENDS) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum += d4.v[i];
+                } else {
+                    float* py = &sy[buf][ch * DS + t];
+                    if constexpr (P == 16) {
+                        const bool up8 = (tid & 8) != 0, up4 = (tid & 4) != 0;
+                        const float a = dpp_choose<kRor8>(up8, out[0], out[1]), c = dpp_choose<kRor8>(up8, out[2], out[3]);
+                        const float v = dpp_choose<kHalfMirror>(up4, a, c);
+                        py[reduced_position<16>(tid)] = dpp_add<kXor2>(dpp_add<kXor1>(v));
+                    } else if constexpr (P == 8) {
+                        const bool up4 = (tid & 4) != 0;
+                        const float a = dpp_choose<kHalfMirror>(up4, out[0], out[1]), c = dpp_choose<kHalfMirror>(up4, out[2], out[3]);
+                        py[reduced_position<8>(tid)] = dpp_add<kXor2>(dpp_add<kXor1>(a));
+                        py[2 + reduced_position<8>(tid)] = dpp_add<kXor2>(dpp_add<kXor1>(c));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (P >= 2) out[i] = dpp_add<kXor1>(out[i]);
+                            if constexpr (P >= 4) out[i] = dpp_add<kXor2>(out[i]);
+                        }
+                        store<float, 4>(py, Pack<float, 4>{out[0], out[1], out[2], out[3]});
+                    }
                 }
-                if constexpr (!ENDS) {
-                    if (p == 0) store<float, 4>(&sx[ch * DS + t], Pack<float, 4>{out[0], out[1], out[2], out[3]});
+                d4 = dn;
+                x4 = xn;
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    b4[s] = bn[s];
+                    if constexpr (!ENDS) c4[s] = cn[s];
                 }
             }
         }
+        if (more) stage(next, t0 + TT, buf ^ 1);
+        __syncthreads();
         if constexpr (!ENDS) {
-            __syncthreads();
-            for (int i = tid; i < kTile * CW; i += kScanThreads) {
-                const int t = i / CW, c = i % CW, at = t0 + t;
-                if (at >= end || e0 + c >= E) continue;
-                float o = 0.0f;
-                if (at < stop) {
-                    o = sx[c * DS + t];
-                    if (q.d) o = __builtin_fmaf(q.d[e0 + c], (float)x[at * q.x_r + e0 + c], o);
-                    if (z) o *= silu((float)z[at * q.z_r + e0 + c]);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const int tt = (j * kScanThreads + tid) / CQ, at = t0 + tt;
+                if (at >= end || e0 + cq >= E) continue;
+                Pack<T, 4> o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = 0.0f;
+                    if (at < stop) {
+                        v = __builtin_fmaf(dcoef[i], now.x[j][i], sy[buf][(cq + i) * DS + tt]);
+                        if (q.gate) v *= silu(now.z[j][i]);
+                    }
+                    o.v[i] = (T)v;
                 }
-                y[(int64_t)at * E + e0 + c] = (T)o;
+                T* to = y + (int64_t)at * E + e0 + cq;
+                if constexpr (V == 4) {
+                    store<T, 4>(to, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (e0 + cq + i < E) to[i] = o.v[i];
+                }
             }
         }
+        now = next;
     }
     if (!mine) return;
     if constexpr (ENDS) {
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (p * S + s < q.n) kept[(piece + 1) * kept_step + p * S + s] = h[s];
+            if (s * P + p < q.n) q.states[((b * (q.pieces + 1) + piece + 1) * q.n + s * P + p) * E + e] = h[s];
         if (p == 0) q.steps[(b * q.pieces + piece) * E + e] = sum;
     } else if (piece == last_piece) {
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (p * S + s < q.n) q.state_out[(b * E + e) * q.n + p * S + s] = h[s];
+            if (s * P + p < q.n) q.state_out[(b * E + e) * q.n + s * P + p] = h[s];
     }
 }
 
-// How a call is cut: pieces of piece_len positions (a multiple of kTile).
+// P = 1, 2 or 4 adjacent lanes own a channel, each N of its states (n = p N + k); a wave walks the positions of its piece by itself.  B[t] and
+// C[t] are the same for all channels and come from LDS, so that a state costs five instructions (two products, exp, two fused) and only one
+// sum over P lanes crosses them; steps and gates are worked out by each of the P.  All loads
+// are kAhead positions ahead; each wave has LDS of its own, so no barrier is needed; four of
+// them make a workgroup only because its waves are dealt out evenly over a CU's SIMDs.
+constexpr int kAhead = 8;
+
+template <class T, int N, int P, bool ENDS>
+__global__ __launch_bounds__(kScanThreads) void scan_lane_kernel(ScanArgs q) {
+    constexpr int NP = N * P, W = ENDS ? NP : 2 * NP, CW = 64 / P, RB = (kAhead * W + 63) / 64;       // values of B (and C) for each position; loads of each lane
+    __shared__ alignas(16) float lds[kScanThreads / 64][2][kAhead * W];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float(*rows)[kAhead * W] = lds[wave];
+    int64_t id = block_index() * (kScanThreads / 64) + wave;
+    if (id >= q.blocks) return;
+    const int group = (int)(id % q.groups);
+    id /= q.groups;
+    const int piece = (int)(id % q.pieces);
+    const int64_t b = id / q.pieces;
+    const int lane = threadIdx.x & 63, p = lane % P, n0 = p * N, E = q.channels, e = group * CW + lane / P, ec = min(e, E - 1);
+    const bool mine = e < E;
+    const int n = q.lengths ? min(max(q.lengths[b], 0), q.len) : q.len;
+    const int begin = piece * q.piece_len, end = min(begin + q.piece_len, q.len), stop = min(end, n);
+    const int last_piece = n > 0 ? (n - 1) / q.piece_len : 0;
+    float a2[N], h[N];
+    const float* start = ENDS || q.pieces == 1 ? (piece == 0 ? q.state : nullptr) : nullptr;
+    const float* kept = q.pieces > 1 ? q.states + ((b * (q.pieces + 1) + piece) * q.n) * E + ec : nullptr;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int kc = min(n0 + k, q.n - 1);
+        const bool real = n0 + k < q.n;
+        a2[k] = real ? q.a[(int64_t)ec * q.n + kc] * kLog2e : 0.0f;
+        h[k] = 0.0f;
+        if (start) h[k] = real ? start[(b * E + ec) * q.n + kc] : 0.0f;
+        if (!ENDS && kept) h[k] = real ? kept[(int64_t)kc * E] : 0.0f;
+    }
+    const float bias = q.dt_bias ? q.dt_bias[ec] : 0.0f, dcoef = !ENDS && q.d ? q.d[ec] : 0.0f;
+    float sum = 0.0f;
+    const T* x = (const T*)q.x + b * q.x_b;
+    const T* dt = (const T*)q.dt + b * q.dt_b;
+    const T* z = (const T*)q.z + b * q.z_b;
+    const T* bm = (const T*)q.b + b * q.b_b;
+    const T* cm = (const T*)q.c + b * q.c_b;
+    T* y = (T*)q.y + b * q.len * (int64_t)E;
+    struct Raw {
+        Loaded<T, 0> x[kAhead], dt[kAhead], z[kAhead], bc[RB];
+    };
+    auto fetch = [&](Raw& r, int t0) {           // rows at or behind `stop` repeat the last one in front of it
+        const T *px = x + t0 * q.x_r, *pd = dt + t0 * q.dt_r, *pz = z + t0 * q.z_r;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            r.x[i].from(px, ec, E);
+            r.dt[i].from(pd, ec, E);
+            if constexpr (!ENDS) {
+                if (q.gate) r.z[i].from(pz, ec, E);
+            }
+            if (t0 + i + 1 < stop) {
+                px += q.x_r;
+                pd += q.dt_r;
+                pz += q.z_r;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            const int i = j * 64 + lane, k = i % NP;
+            const int64_t t = min(t0 + min(i / W, kAhead - 1), stop - 1);
+            const T* row = !ENDS && i / NP % 2 ? cm + t * q.c_r : bm + t * q.b_r;
+            r.bc[j].from(row, k, q.n);
+        }
+    };
+    auto stage = [&](const Raw& r, int buf) {
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            const int i = j * 64 + lane;
+            if (kAhead * W % 64 == 0 || i < kAhead * W) rows[buf][i] = i % NP < q.n ? r.bc[j][0] : 0.0f;
+        }
+    };
+    Raw now, next;
+#pragma unroll
+    for (int k = 0; k < N; ++k) asm volatile("" : "+v"(h[k]), "+v"(a2[k]));
+    // `count` positions from t0 on: steps and gates first, then the states without a branch between positions, then the results
+    auto block = [&](int t0, int count, int buf) {
+        float d[kAhead], dx[kAhead], out[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) d[i] = now.dt[i][0] + bias;
+        if (q.softplus) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float xv = now.x[i][0];
+            dx[i] = d[i] * xv;
+            out[i] = P == 1 || p == 0 ? dcoef * xv : 0.0f;
+            if constexpr (ENDS) sum += i < count ? d[i] : 0.0f;
+        }
+        // G states at a time: their products, exps, products and fused adds each as G instructions in a row, so that none waits for the one in
+        // front of it; the next group's B and C are read meanwhile.  The fences keep the compiler from mixing them again.
+        constexpr int G = N < 8 ? N : 8, GROUPS = N / G;
+        float bv[2][G], cv[2][G];
+        auto read = [&](int at, int to) {
+            const float* row = &rows[buf][at / GROUPS * W + n0 + at % GROUPS * G];
+#pragma unroll
+            for (int k = 0; k < G; k += 4) {
+                const Pack<float, 4> p = load<float, 4>(row + k);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) bv[to][k + c] = p.v[c];
+                if constexpr (!ENDS) {
+                    const Pack<float, 4> r = load<float, 4>(row + NP + k);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) cv[to][k + c] = r.v[c];
+                }
+            }
+        };
+        read(0, 0);
+#pragma unroll
+        for (int at = 0; at < kAhead * GROUPS; ++at) {
+            const int i = at / GROUPS, k0 = at % GROUPS * G;
+            if (i >= count) break;
+            if (at + 1 < kAhead * GROUPS) read(at + 1, (at + 1) & 1);
+            float g[G], u[G];
+#pragma unroll
+            for (int k = 0; k < G; ++k) g[k] = d[i] * a2[k0 + k];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < G; ++k) g[k] = __builtin_amdgcn_exp2f(g[k]);
+#pragma unroll
+            for (int k = 0; k < G; ++k) u[k] = dx[i] * bv[at & 1][k];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < G; ++k) h[k0 + k] = __builtin_fmaf(g[k], h[k0 + k], u[k]);
+            if constexpr (!ENDS) {
+                float part[4] = {out[i], 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < G; ++k) part[k & 3] = k < 4 && k > 0 ? h[k0 + k] * cv[at & 1][k] : __builtin_fmaf(h[k0 + k], cv[at & 1][k], part[k & 3]);
+                out[i] = (part[0] + part[1]) + (part[2] + part[3]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!ENDS) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if constexpr (P >= 2) out[i] = dpp_add<kXor1>(out[i]);
+                if constexpr (P >= 4) out[i] = dpp_add<kXor2>(out[i]);
+            }
+            if (q.gate) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) out[i] *= silu(now.z[i][0]);
+            }
+            if (mine && p == 0) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+                    if (i < count) y[(int64_t)(t0 + i) * E + e] = (T)out[i];
+            }
+        }
+    };
+    int buf = 0;
+    if (begin < stop) {
+        fetch(now, begin);
+        stage(now, 0);
+    }
+    int t0 = begin;
+    for (; t0 + kAhead <= stop; t0 += kAhead) {
+        const bool more = t0 + kAhead < stop;
+        if (more) fetch(next, t0 + kAhead);
+        block(t0, kAhead, buf);
+        if (more) stage(next, buf ^ 1);
+        buf ^= 1;
+        now = next;
+    }
+    if (t0 < stop) block(t0, stop - t0, buf);
+    if (!mine) return;
+    if constexpr (ENDS) {
+        float* to = q.states + ((b * (q.pieces + 1) + piece + 1) * q.n) * E + e;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (n0 + k < q.n) to[(int64_t)(n0 + k) * E] = h[k];
+        if (p == 0) q.steps[(b * q.pieces + piece) * E + e] = sum;
+    } else {
+        for (int t = max(begin, stop) + p; t < end; t += P) y[(int64_t)t * E + e] = (T)0.0f;
+        if (piece == last_piece) {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (n0 + k < q.n) q.state_out[(b * E + e) * q.n + n0 + k] = h[k];
+        }
+    }
+}
+
+// The state in front of every piece from those behind them: slot k of `states` holds what piece k - 1 left (slot 0 nothing yet), and gets
+// what piece k starts from.  The first piece has started from `state`.
+__global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs q, int64_t count) {
+    const int64_t i = block_index() * kScanThreads + threadIdx.x;
+    if (i >= count) return;
+    const int E = q.channels, e = (int)(i % E), k = (int)(i / E % q.n);
+    const int64_t b = i / E / q.n, step = (int64_t)E * q.n;
+    const float a2 = q.a[(int64_t)e * q.n + k] * kLog2e;
+    float* slot = q.states + (b * (q.pieces + 1) * q.n + k) * E + e;
+    const float* sums = q.steps + b * q.pieces * E + e;
+    float h = q.state ? q.state[(b * E + e) * q.n + k] : 0.0f;
+    slot[0] = h;
+    h = slot[step];
+    constexpr int A = 8;
+    for (int j0 = 1; j0 < q.pieces; j0 += A) {
+        float sum[A], part[A];
+#pragma unroll
+        for (int j = 0; j < A; ++j) {
+            const int64_t at = min(j0 + j, q.pieces - 1);
+            sum[j] = sums[at * E];
+            part[j] = slot[(at + 1) * step];
+        }
+#pragma unroll
+        for (int j = 0; j < A; ++j) {
+            if (j0 + j < q.pieces) {
+                slot[(j0 + j) * step] = h;
+                h = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[j] * a2), h, part[j]);
+            }
+        }
+    }
+}
+
+// One position: bound by reading and writing the states.  P lanes share a channel, each holds V adjacent states; they keep A in registers
+// and walk `each` sequences.
+template <class T, int P, int V>
+__global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int batch, int each) {
+    constexpr int CW = kScanThreads / P;
+    const int64_t id = block_index();
+    if (id >= q.blocks) return;
+    const int tid = threadIdx.x, p = tid % P, e = (int)(id % q.groups) * CW + tid / P, E = q.channels;
+    const int b0 = (int)(id / q.groups) * each, b1 = min(b0 + each, batch);
+    const int k = p * V;                         // V = 4: states are whole groups of four
+    if (e >= E) return;                          // whole groups of lanes that share a channel
+    const bool mine = k < q.n;
+    Pack<float, V> a2{};
+    if (mine) a2 = load<float, V>(q.a + (int64_t)e * q.n + k);
+    const float bias = q.dt_bias ? q.dt_bias[e] : 0.0f, dcoef = q.d ? q.d[e] : 0.0f;
+    for (int b = b0; b < b1; ++b) {
+        const int64_t at = ((int64_t)b * E + e) * q.n + k;
+        Pack<float, V> h{};
+        if (mine && q.state) h = load<float, V>(q.state + at);
+        float out = 0.0f;
+        if (!q.lengths || q.lengths[b] > 0) {
+            const float x = (float)((const T*)q.x)[b * q.x_b + e];
+            float d = (float)((const T*)q.dt)[b * q.dt_b + e] + bias;
+            if (q.softplus) d = softplus(d);
+            if (mine) {
+                const Pack<T, V> bm = load<T, V>((const T*)q.b + b * q.b_b + k), cm = load<T, V>((const T*)q.c + b * q.c_b + k);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    h.v[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * (a2.v[i] * kLog2e)), h.v[i], d * x * (float)bm.v[i]);
+                    out = __builtin_fmaf(h.v[i], (float)cm.v[i], out);
+                }
+            }
+            out = lanes_sum<P>(out);
+            out = __builtin_fmaf(dcoef, x, out);
+            if (q.gate) out *= silu((float)((const T*)q.z)[b * q.z_b + e]);
+        }
+        if (p == 0) ((T*)q.y)[(int64_t)b * E + e] = (T)out;
+        if (mine) store<float, V>(q.state_out + at, h);
+    }
+}
+
+template <class T, int V>
+static int launch_step(ScanArgs a, int batch, hipStream_t st) {
+    int lanes = 1;
+    while (lanes * V < a.n) lanes *= 2;
+    a.groups = (int)ceil_div(a.channels, kScanThreads / lanes);
+    // up to four sequences for each workgroup, so that A is read once for them, as long as 1024 workgroups remain
+    const int each = (int)std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)a.groups * batch / 1024));
+    a.blocks = a.groups * ceil_div(batch, each);
+    if (a.blocks > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "selective_scan: the batch is too large for one call");
+    const dim3 grid = grid_of(a.blocks), block(kScanThreads);
+    switch (lanes) {
+        case 1: hipLaunchKernelGGL((scan_step_kernel<T, 1, V>), grid, block, 0, st, a, batch, each); break;
+        case 2: hipLaunchKernelGGL((scan_step_kernel<T, 2, V>), grid, block, 0, st, a, batch, each); break;
+        case 4: hipLaunchKernelGGL((scan_step_kernel<T, 4, V>), grid, block, 0, st, a, batch, each); break;
+        case 8: hipLaunchKernelGGL((scan_step_kernel<T, 8, V>), grid, block, 0, st, a, batch, each); break;
+        case 16: hipLaunchKernelGGL((scan_step_kernel<T, 16, V>), grid, block, 0, st, a, batch, each); break;
+        case 32: hipLaunchKernelGGL((scan_step_kernel<T, 32, V>), grid, block, 0, st, a, batch, each); break;
+        default: hipLaunchKernelGGL((scan_step_kernel<T, 64, V>), grid, block, 0, st, a, batch, each); break;
+    }
+    return TAE_OK;
+}
+
+// How a call is cut: P lanes for a channel, each with S states, by scan_lane_kernel or (tiled) selective_scan_kernel, and pieces.
 struct ScanPlan {
-    int lanes = 1, per_lane = 4, groups = 1, pieces = 1, piece_len = 0;
+    int lanes = 1, per_lane = 1, tiled = 0, groups = 1, pieces = 1, piece_len = 0;
     size_t steps_bytes = 0, bytes = 0;
 };
 
-static bool plan_scan(const tae_scan_args* p, ScanPlan* s) {
-    if (p->batch < 1 || p->len < 1 || p->channels < 1 || p->states < 1 || p->states > 64) return false;
-    while (s->per_lane * s->lanes < p->states) s->lanes *= 2;
-    s->groups = (int)ceil_div(p->channels, kScanThreads / s->lanes);
-    const int64_t wgs = (int64_t)p->batch * s->groups;
-    int64_t pieces = 1;
-    if (wgs < 128) pieces = std::min<int64_t>(ceil_div(256, wgs), ceil_div(p->len, 4 * kTile));
-    s->piece_len = (int)(ceil_div(ceil_div(p->len, pieces), kTile) * kTile);
-    s->pieces = (int)ceil_div(p->len, s->piece_len);
-    if (s->pieces > 1) {
-        s->steps_bytes = ((size_t)p->batch * s->pieces * p->channels * 4 + 255) / 256 * 256;
-        s->bytes = s->steps_bytes + (size_t)p->batch * (s->pieces + 1) * p->channels * p->states * 4;
+constexpr int kPieceUnit = 64;                   // pieces are whole tiles
+
+// Few channels leave SIMDs empty: then fewer states for each lane, or pieces along the positions, which cost a second pass (ENDS).  The
+// choice is the cheapest by the time that a wave takes for one position, times the positions and the waves that a SIMD (1024 of them) runs.
+// Measured: a vector instruction issues every 2.0 ns, an exp every 4.4, and a single wave reaches half of that, so one wave takes as long as
+// two.  A state takes four instructions and an exp, 12.4 ns (three in the ends pass, 10.4); the softplus, gate and D of a channel 55 ns (ends
+// pass: 30), by every lane of a channel in scan_lane_kernel, shared by its P lanes in the tiled one, which adds about 18 for sums over lanes,
+// LDS and barriers.
+static bool plan_scan(const tae_scan_args* p, ScanPlan* out) {
+    if (p->batch < 1 || p->len < 1 || p->channels < 1 || p->states < 1 || p->states > 64 || !dtype_ok(p->dtype)) return false;
+    if (p->len == 1) return true;
+    int padded = 4;
+    while (padded < p->states) padded *= 2;
+    double least = 0.0;
+    for (int form = 0; form < 8; ++form) {
+        const int tiled = form >= 3, lanes = tiled ? 1 << (form - 3) : 1 << form, per_lane = padded / lanes;
+        if (lanes > padded || (tiled ? per_lane > 4 : per_lane < 4 || per_lane > 32)) continue;
+        const int64_t groups = ceil_div(p->channels, tiled ? kScanThreads / lanes : 64 / lanes), waves = tiled ? 4 : 1;
+        const double channel = tiled ? 1.0 / lanes : 1.0, across = tiled ? 18.0 : lanes > 1 ? 4.0 : 0.0;
+        for (int64_t pieces = 1; pieces <= 64; ++pieces) {
+            const int64_t piece_len = ceil_div(ceil_div(p->len, pieces), kPieceUnit) * kPieceUnit;
+            if (ceil_div(p->len, piece_len) < pieces) continue;
+            // waves of a SIMD, three at a time at the most; a wave starts with about 3 us of loads
+            auto time = [&](int64_t n, double ns) {
+                const double all = std::ceil(n * waves * p->batch * groups / 1024.0 * 4.0) / 4.0, whole = std::floor(all / 3.0), rest = all - 3.0 * whole;
+                return (3.0 * whole + (rest > 0.0 ? std::max(2.0, rest) : 0.0)) * std::min<int64_t>(piece_len, p->len) * ns + (whole + (rest > 0.0)) * 3000.0;
+            };
+            double cost = time(pieces, 12.4 * per_lane + 55.0 * channel + across);
+            if (pieces > 1) cost += time(pieces - 1, 10.4 * per_lane + 30.0 * channel + across) + 9000.0;
+            if (least == 0.0 || cost < least) {
+                least = cost;
+                out->lanes = lanes;
+                out->per_lane = per_lane;
+                out->tiled = tiled;
+                out->groups = (int)groups;
+                out->pieces = (int)pieces;
+                out->piece_len = (int)piece_len;
+            }
+        }
+    }
+    if (out->pieces > 1) {
+        out->steps_bytes = ((size_t)p->batch * out->pieces * p->channels * 4 + 255) / 256 * 256;
+        out->bytes = out->steps_bytes + (size_t)p->batch * (out->pieces + 1) * p->channels * p->states * 4;
     }
     return true;
 }
 
-template <class T, int P>
-static void launch_scan(const ScanArgs& a, hipStream_t st) {
-    if (a.pieces > 1) hipLaunchKernelGGL((selective_scan_kernel<T, 4, P, true>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
-    hipLaunchKernelGGL((selective_scan_kernel<T, 4, P, false>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
+static void launch_join(const ScanArgs& a, int64_t batch, hipStream_t st) {
+    const int64_t count = batch * a.n * a.channels;
+    hipLaunchKernelGGL(scan_join_kernel, grid_of(ceil_div(count, kScanThreads)), dim3(kScanThreads), 0, st, a, count);
+}
+
+template <class T, int S, int P, int TT, int V>
+static void launch_scan_as(const ScanArgs& a, int64_t batch, hipStream_t st) {
+    if (a.pieces > 1) {
+        hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, true>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
+        launch_join(a, batch, st);
+    }
+    hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, false>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
+}
+
+template <class T, int S, int P, int TT>
+static int launch_scan(const ScanArgs& a, bool vector, int64_t batch, hipStream_t st) {
+    vector ? launch_scan_as<T, S, P, TT, 4>(a, batch, st) : launch_scan_as<T, S, P, TT, 1>(a, batch, st);
+    return TAE_OK;
+}
+
+template <class T, int N, int P>
+static int launch_lane(const ScanArgs& a, int64_t batch, hipStream_t st) {
+    const dim3 grid = grid_of(ceil_div(a.blocks, kScanThreads / 64));
+    if (a.pieces > 1) {
+        hipLaunchKernelGGL((scan_lane_kernel<T, N, P, true>), grid, dim3(kScanThreads), 0, st, a);
+        launch_join(a, batch, st);
+    }
+    hipLaunchKernelGGL((scan_lane_kernel<T, N, P, false>), grid, dim3(kScanThreads), 0, st, a);
+    return TAE_OK;
 }
 
 template <class T>
-static void launch_scan_lanes(const ScanArgs& a, int lanes, hipStream_t st) {
-    switch (lanes) {
-        case 1: launch_scan<T, 1>(a, st); break;
-        case 2: launch_scan<T, 2>(a, st); break;
-        case 4: launch_scan<T, 4>(a, st); break;
-        case 8: launch_scan<T, 8>(a, st); break;
-        default: launch_scan<T, 16>(a, st); break;
+static int launch_scan_plan(const ScanArgs& a, const ScanPlan& s, bool v, int batch, hipStream_t st) {
+    if (a.len == 1) return v ? launch_step<T, 4>(a, batch, st) : launch_step<T, 1>(a, batch, st);
+    switch (s.tiled * 10000 + s.lanes * 100 + s.per_lane) {
+        case 104: return launch_lane<T, 4, 1>(a, batch, st);
+        case 108: return launch_lane<T, 8, 1>(a, batch, st);
+        case 116: return launch_lane<T, 16, 1>(a, batch, st);
+        case 132: return launch_lane<T, 32, 1>(a, batch, st);
+        case 204: return launch_lane<T, 4, 2>(a, batch, st);
+        case 208: return launch_lane<T, 8, 2>(a, batch, st);
+        case 216: return launch_lane<T, 16, 2>(a, batch, st);
+        case 232: return launch_lane<T, 32, 2>(a, batch, st);
+        case 404: return launch_lane<T, 4, 4>(a, batch, st);
+        case 408: return launch_lane<T, 8, 4>(a, batch, st);
+        case 416: return launch_lane<T, 16, 4>(a, batch, st);
+        case 10104: return launch_scan<T, 4, 1, 16>(a, v, batch, st);
+        case 10202: return launch_scan<T, 2, 2, 16>(a, v, batch, st);
+        case 10204: return launch_scan<T, 4, 2, 16>(a, v, batch, st);
+        case 10401: return launch_scan<T, 1, 4, 32>(a, v, batch, st);
+        case 10402: return launch_scan<T, 2, 4, 32>(a, v, batch, st);
+        case 10404: return launch_scan<T, 4, 4, 32>(a, v, batch, st);
+        case 10801: return launch_scan<T, 1, 8, 32>(a, v, batch, st);
+        case 10802: return launch_scan<T, 2, 8, 32>(a, v, batch, st);
+        case 10804: return launch_scan<T, 4, 8, 32>(a, v, batch, st);
+        case 11601: return launch_scan<T, 1, 16, 64>(a, v, batch, st);
+        case 11602: return launch_scan<T, 2, 16, 64>(a, v, batch, st);
+        case 11604: return launch_scan<T, 4, 16, 64>(a, v, batch, st);
     }
+    return fail_msg(TAE_EINVAL, "internal: selective_scan has no kernel for this plan");
 }
 
 }  // namespace seq
@@ -210,19 +742,27 @@ int tae_selective_scan(const tae_scan_args* p, void* stream) {
     if (!plan_scan(p, &s)) return fail_msg(TAE_EINVAL, "selective_scan: bad sizes");
     if (s.bytes && (!p->workspace || p->workspace_bytes < s.bytes || !aligned(p->workspace, 16)))
         return fail_msg(TAE_EINVAL, "selective_scan: the workspace is missing, misaligned or smaller than tae_selective_scan_workspace");
-    ScanArgs a{p->x, p->dt, p->b, p->c, p->z, p->a, p->d, p->dt_bias, p->state, p->lengths, p->y, p->state_out,
+    ScanArgs a{p->x, p->dt, p->b, p->c, p->z ? p->z : p->x, p->a, p->d, p->dt_bias, p->state, p->lengths, p->y, p->state_out,
                s.bytes ? (float*)p->workspace : nullptr, s.bytes ? (float*)((char*)p->workspace + s.steps_bytes) : nullptr,
-               p->x_batch, p->x_row, p->dt_batch, p->dt_row, p->b_batch, p->b_row, p->c_batch, p->c_row, p->z_batch, p->z_row,
-               p->len, p->channels, p->states, p->softplus ? 1 : 0, s.groups, s.pieces, s.piece_len, (int64_t)p->batch * s.groups * s.pieces};
+               p->x_batch, p->x_row, p->dt_batch, p->dt_row, p->b_batch, p->b_row, p->c_batch, p->c_row, p->z ? p->z_batch : p->x_batch, p->z ? p->z_row : p->x_row,
+               p->len, p->channels, p->states, p->softplus ? 1 : 0, p->z ? 1 : 0, s.groups, s.pieces, s.piece_len, (int64_t)p->batch * s.groups * s.pieces};
+    const size_t four = 4 * dtype_bytes(p->dtype);
+    Width w(dtype_bytes(p->dtype));
+    w.elements(p->channels).pointer(p->x).pointer(p->dt).pointer(p->z).pointer(p->y).elements(p->x_batch).elements(p->x_row).elements(p->dt_batch).elements(p->dt_row);
+    if (p->z) w.elements(p->z_batch).elements(p->z_row);
+    Width w4(4);
+    w4.elements(p->states).pointer(p->a).pointer(p->state).pointer(p->state_out);
+    Width wb(dtype_bytes(p->dtype));
+    wb.pointer(p->b).pointer(p->c).elements(p->b_batch).elements(p->c_batch);
+    const bool vector = p->len > 1 ? w.fits(four) : w4.fits(16) && wb.fits(four);      // one position: of the states and of B and C
     if (a.blocks > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "selective_scan: the batch is too large for one call");
     return guarded([&] {
         hipStream_t st = (hipStream_t)stream;
         switch (p->dtype) {
-            case TAE_DTYPE_F32: launch_scan_lanes<float>(a, s.lanes, st); break;
-            case TAE_DTYPE_F16: launch_scan_lanes<f16>(a, s.lanes, st); break;
-            default: launch_scan_lanes<bf16>(a, s.lanes, st); break;
+            case TAE_DTYPE_F32: return launch_scan_plan<float>(a, s, vector, p->batch, st);
+            case TAE_DTYPE_F16: return launch_scan_plan<f16>(a, s, vector, p->batch, st);
+            default: return launch_scan_plan<bf16>(a, s, vector, p->batch, st);
         }
-        return (int)TAE_OK;
     });
 }
 
