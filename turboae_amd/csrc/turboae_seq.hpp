@@ -42,18 +42,34 @@ __device__ __forceinline__ float softplus(float x) {
     return fmaxf(x, 0.0f) + __builtin_fmaf(__builtin_amdgcn_logf(u), kLn2, w - (u - 1.0f));
 }
 
-// sums and maxima over the 2^k adjacent lanes that share a value (W a power of two up to 64)
-template <int W>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-    for (int o = 1; o < W; o <<= 1) v += __shfl_xor(v, o, 64);
+// A value from another lane of the same 16: quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror, row_mirror, row_ror:8.  All lanes that take part
+// have to be active: never inside a choice that lanes make differently.
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140, kRor8 = 0x128;
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float lane_value(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+
+// `op` over the W adjacent lanes that share a value (W a power of two up to 64); every lane gets the result.  The mirrors pair lanes that
+// already hold the same partial result.
+template <int W, class Op>
+__device__ __forceinline__ float lanes_join(float v, Op&& op) {
+    if constexpr (W >= 2) v = op(v, dpp<kXor1>(v));
+    if constexpr (W >= 4) v = op(v, dpp<kXor2>(v));
+    if constexpr (W >= 8) v = op(v, dpp<kHalfMirror>(v));
+    if constexpr (W >= 16) v = op(v, dpp<kMirror>(v));
+    if constexpr (W == 32) v = op(v, __shfl_xor(v, 16, 64));
+    if constexpr (W == 64) v = op(op(lane_value(v, 0), lane_value(v, 16)), op(lane_value(v, 32), lane_value(v, 48)));
     return v;
 }
 template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return lanes_join<W>(v, [](float a, float b) { return a + b; });
+}
+template <int W>
 __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-    for (int o = 1; o < W; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    return lanes_join<W>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 inline size_t dtype_bytes(int32_t t) { return t == TAE_DTYPE_F32 ? 4 : 2; }

@@ -35,23 +35,33 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
 
+template <int CTRL>
+__device__ __forceinline__ u64 dpp_key(u64 k) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)k, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(k >> 32), CTRL, 0xF, 0xF, true);
+    return ((u64)hi << 32) | lo;
+}
 template <int W>
 __device__ __forceinline__ u64 lanes_max_key(u64 k) {
-#pragma unroll
-    for (int o = 1; o < W; o <<= 1) {
-        const u64 other = __shfl_xor(k, o, 64);
-        k = other > k ? other : k;
+    auto op = [](u64 a, u64 b) { return a > b ? a : b; };
+    k = op(k, dpp_key<kXor1>(k));
+    k = op(k, dpp_key<kXor2>(k));
+    k = op(k, dpp_key<kHalfMirror>(k));
+    if constexpr (W == 64) {
+        k = op(k, dpp_key<kMirror>(k));
+        k = op(k, __shfl_xor(k, 16, 64));
+        k = op(k, __shfl_xor(k, 32, 64));
     }
+    static_assert(W == 8 || W == 64, "lanes of a row");
     return k;
 }
 
 struct Stats {
     float m, s, t;
 };
-// Rescaled to the larger maximum.  A factor of 0 takes its part away whatever its t (a mask of the type's lowest value has an infinite one),
-// but not a NaN of its s.
+// Rescaled to the larger maximum.  A factor of 0 takes its part away whatever its t (a mask of the type's lowest value has an infinite one).
+// A row with a NaN has the maximum NaN.
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
-    const float m = fmaxf(a.m, b.m);
+    const float m = __builtin_elementwise_maximum(a.m, b.m);
     const float da = a.m == kNegInf ? kNegInf : a.m - m, db = b.m == kNegInf ? kNegInf : b.m - m;
     const float fa = exp_fast(da), fb = exp_fast(db);
     const float ta = fa == 0.0f ? 0.0f : __builtin_fmaf(da, a.s, a.t) * fa, tb = fb == 0.0f ? 0.0f : __builtin_fmaf(db, b.s, b.t) * fb;
@@ -88,57 +98,112 @@ __device__ __forceinline__ void write_top(const LogprobsArgs& a, int64_t row, in
     a.top_logp[row * a.top + i] = none ? __builtin_nanf("") : st.m == kNegInf ? kNegInf : key_value(key) - st.m - log_s;
 }
 
-// W lanes (64 or fewer: a share of a wave; more: the workgroup) read a part of up to W * EPT - 15 elements.
-template <class T, int W, int EPT, int THREADS>
+__device__ __forceinline__ uint32_t order_of(u64 k) { return (uint32_t)(k >> 32); }
+
+// W lanes (64 or fewer: a share of a wave; more: the workgroup) read a part of a row into registers, EPT elements each, in granules of V.
+//
+// Alternatives: `top` lanes of a wave have a largest element at or above the wave's top-th largest lane maximum, so no element below the
+// largest of these bounds over the waves is among the `top` (the bound is cut to 16 bits, which only lowers it).  What is at or above it, a few
+// dozen elements of a usual row, is collected in LDS in any order and sorted by counting larger keys.  Rows with more than fit (many equal
+// values) take the largest one by one.
+template <class T, int W, int EPT, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) {
-    constexpr int V = 16 / sizeof(T), G = EPT / V, WAVES = W > 64 ? W / 64 : 1;
-    __shared__ float lds_f[16][3];
-    __shared__ u64 lds_k[2][16];
+    constexpr int G = EPT / V, WAVES = W > 64 ? W / 64 : 1, WW = W < 64 ? W : 64, ROOM = W < 64 ? 1 : 128;
+    __shared__ float lds_f[WAVES][3];
+    __shared__ u64 lds_k[2][WAVES], found[WAVES][ROOM];
+    __shared__ uint32_t lds_u[WAVES], lds_n[WAVES];
     const int lane = threadIdx.x % W;
     const int64_t unit = block_index() * (THREADS / W) + threadIdx.x / W;
-    if (unit >= (int64_t)a.rows * a.parts) return;                  // whole workgroups, or lanes of W <= 64, which meet no barrier
+    if (unit >= (int64_t)a.rows * a.parts) return;                  // whole workgroups, or lanes of W < 64, which meet no barrier
     const int64_t row = unit / a.parts;
     const int part = (int)(unit % a.parts);
     const int lo = part * a.part_len, hi = min(lo + a.part_len, a.vocab);
     const T* x = (const T*)a.logits + row * a.row;
-    // 16-byte granules in step with the addresses; elements in front of lo or behind hi in the outermost ones are not touched
-    const int skew = (int)(reinterpret_cast<uintptr_t>(x + lo) / sizeof(T) % V);
-    Pack<T, V> r[G];
+    // granules in step with 16-byte addresses
+    const int skew = V == 1 ? 0 : (int)(reinterpret_cast<uintptr_t>(x + lo) / sizeof(T) % V);
+    auto place = [&](int g) { return lo - skew + (g * W + lane) * V; };
+    // as whole registers, taken apart anew in each pass over them (`again` keeps the compiler from holding the parts)
+    constexpr int D = V == 1 ? 1 : 4;            // registers of a granule
+    uint32_t w[G][D];
+    auto value = [&](int g, int i) -> float {
+        if constexpr (V == 1 || sizeof(T) == 4) return __uint_as_float(w[g][i]);
+        else return (float)__builtin_bit_cast(T, (uint16_t)(i & 1 ? w[g][i / 2] >> 16 : w[g][i / 2] & 0xFFFFu));
+    };
+    auto again = [&]() {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const int at = lo - skew + (g * W + lane) * V;
-        if (at >= lo && at + V <= hi) {
-            r[g] = load<T, V>(x + at);
-        } else {
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int i = 0; i < V; ++i) r[g].v[i] = at + i >= lo && at + i < hi ? x[at + i] : (T)kNegInf;
+            for (int i = 0; i < D; ++i) asm volatile("" : "+v"(w[g][i]));
+    };
+    if constexpr (V == 1) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) w[g][0] = __float_as_uint(place(g) < hi ? (float)x[place(g)] : kNegInf);
+    } else {
+        // whole granules first, all loads in flight at once (others repeat one), then the elements of the outermost ones
+        const int low = lo + (V - skew) % V, high = lo - skew + (hi - lo + skew) / V * V - V;
+        if (high >= low) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint4 u = *reinterpret_cast<const uint4*>(x + min(max(place(g), low), high));
+                w[g][0] = u.x, w[g][1] = u.y, w[g][2] = u.z, w[g][3] = u.w;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int at = place(g);
+            if (at < low || at > high) {
+                Pack<T, V> p;
+#pragma unroll
+                for (int i = 0; i < V; ++i) p.v[i] = at + i >= lo && at + i < hi ? x[at + i] : (T)kNegInf;
+                const uint4 u = __builtin_bit_cast(uint4, p);
+                w[g][0] = u.x, w[g][1] = u.y, w[g][2] = u.z, w[g][3] = u.w;
+            }
         }
     }
-    float m = kNegInf;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int i = 0; i < V; ++i) m = fmaxf(m, (float)r[g].v[i]);
-    m = lanes_max<(W < 64 ? W : 64)>(m);
+    again();
     const int wave = threadIdx.x >> 6;
+    float mine = kNegInf, of[G];                 // largest of the lane and of its granules; NaN if there is one
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        of[g] = value(g, 0);
+#pragma unroll
+        for (int i = 1; i < V; ++i) of[g] = __builtin_elementwise_maximum(of[g], value(g, i));
+        mine = __builtin_elementwise_maximum(mine, of[g]);
+    }
+    again();
+    float m = lanes_join<WW>(mine, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+    uint32_t bound = 0;
+    if constexpr (W >= 64) {
+        if (a.top) {
+            // the largest 16-bit prefix that `top` lane maxima of this wave reach
+            const uint32_t own = lo - skew + lane * V < hi ? order_of(key_of(mine, 0)) : 0u;
+#pragma unroll
+            for (int bit = 31; bit >= 16; --bit) {
+                const uint32_t with = bound | 1u << bit;
+                if (__popcll(__ballot(own >= with)) >= a.top) bound = with;
+            }
+        }
+    }
     if constexpr (W > 64) {
-        if ((threadIdx.x & 63) == 0) lds_f[wave][0] = m;
+        if ((threadIdx.x & 63) == 0) { lds_f[wave][0] = m; lds_u[wave] = bound; }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) m = fmaxf(m, lds_f[i][0]);
+        for (int i = 0; i < WAVES; ++i) { m = __builtin_elementwise_maximum(m, lds_f[i][0]); bound = max(bound, lds_u[i]); }
     }
+    // e^(x - m) = 2^(x log2 e - m log2 e); -inf (and what is far below m) is taken at 2^-1000 = 0, so that 0 times its distance is 0
     const float base = m == kNegInf ? 0.0f : m;
     float s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float d = (float)r[g].v[i] - base, e = exp_fast(d);
+            const float d = fmaxf((value(g, i) - base) * kLog2e, -1000.0f), e = __builtin_amdgcn_exp2f(d);
             s += e;
-            t += e == 0.0f ? 0.0f : d * e;
+            t = __builtin_fmaf(d, e, t);
         }
-    s = lanes_sum<(W < 64 ? W : 64)>(s);
-    t = lanes_sum<(W < 64 ? W : 64)>(t);
+    again();
+    s = lanes_sum<WW>(s);
+    t = lanes_sum<WW>(t);
     if constexpr (W > 64) {
         if ((threadIdx.x & 63) == 0) { lds_f[wave][1] = s; lds_f[wave][2] = t; }
         __syncthreads();
@@ -146,8 +211,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) { s += lds_f[i][1]; t += lds_f[i][2]; }
     }
-    const Stats st{m, s, t};
-    const bool none = s != s || m == __builtin_inff();
+    const Stats st{m, s, t * kLn2};
+    const bool none = m != m || m == __builtin_inff();
     const float log_s = __builtin_amdgcn_logf(s) * kLn2;
     if (lane == 0) {
         if (a.parts == 1) {
@@ -155,27 +220,77 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
             const int64_t token = token_of<T>(a, row, xt);
             finish_row(a, row, st, log_s, none, xt, token);
         } else {
-            store<float, 4>(a.stats + unit * 4, Pack<float, 4>{m, s, t, 0.0f});
+            store<float, 4>(a.stats + unit * 4, Pack<float, 4>{m, s, st.t, 0.0f});
         }
     }
     if (!a.top) return;
-    // the largest key of this lane's elements that is below `limit`
-    auto best_below = [&](u64 limit) {
-        u64 best = 0;
+    auto put = [&](int j, u64 k) {
+        if (a.parts == 1) write_top(a, row, j, k, st, log_s, none);
+        else a.keys[unit * a.top + j] = k;
+    };
+    if constexpr (W >= 64) {
+        // each wave's own list, filled in the order of granules and lanes; granules without a candidate cost one comparison
+        const float least = bound ? key_value((u64)bound << 32) : kNegInf;
+        uint32_t n = 0;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const int at = lo - skew + (g * W + lane) * V;
+            if (!__any(!(of[g] < least))) continue;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const u64 k = at + i >= lo && at + i < hi ? key_of((float)r[g].v[i], at + i) : 0;
-                best = k > best && k < limit ? k : best;
+                const int at = place(g) + i;
+                const float v = value(g, i);
+                const bool yes = !(v < least) && at >= lo && at < hi;
+                const u64 set = __ballot(yes);
+                const uint32_t slot = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
+                if (yes && slot < ROOM) found[wave][slot] = key_of(v, at);
+                n += __popcll(set);
             }
         }
+        bool fits = n <= ROOM;
+        uint32_t total = n;
+        if constexpr (W > 64) {
+            if ((threadIdx.x & 63) == 0) lds_n[wave] = n;
+            __syncthreads();
+            total = 0;
+            fits = true;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                total += lds_n[i];
+                fits = fits && lds_n[i] <= ROOM;
+            }
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if (fits) {
+            for (int j = total + lane; j < a.top; j += W) put(j, 0);      // a part with fewer elements
+            for (int c = threadIdx.x & 63; c < (int)n; c += 64) {
+                const u64 k = found[wave][c];
+                int rank = 0;
+                for (int u = 0; u < WAVES; ++u) {
+                    const int count = W > 64 ? (int)lds_n[u] : (int)n;
+                    for (int i = 0; i < count; ++i) rank += found[u][i] > k;
+                }
+                if (rank < a.top) put(rank, k);
+            }
+            return;
+        }
+    }
+    // the largest key of this lane's elements that is below `limit`
+    auto best_below = [&](u64 limit) {           // read again, so that this rare way costs the usual one no registers
+        u64 best = 0;
+#pragma unroll 1
+        for (int g = 0; g < G; ++g)
+#pragma unroll 1
+            for (int i = 0; i < V; ++i) {
+                const int at = place(g) + i;
+                const u64 k = at >= lo && at < hi ? key_of((float)x[at], at) : 0;
+                best = k > best && k < limit ? k : best;
+            }
         return best;
     };
     u64 best = best_below(~0ull);
     for (int j = 0; j < a.top; ++j) {
-        u64 k = lanes_max_key<(W < 64 ? W : 64)>(best);
+        u64 k = lanes_max_key<WW>(best);
         if constexpr (W > 64) {
             if ((threadIdx.x & 63) == 0) lds_k[j & 1][wave] = k;
             __syncthreads();
@@ -183,68 +298,87 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
             for (int i = 0; i < WAVES; ++i) k = lds_k[j & 1][i] > k ? lds_k[j & 1][i] : k;
         }
         if (best == k) best = best_below(k);     // keys differ, so one lane (or, with none left, all of them)
-        if (lane == 0) {
-            if (a.parts == 1) write_top(a, row, j, k, st, log_s, none);
-            else a.keys[unit * a.top + j] = k;
-        }
+        if (lane == 0) put(j, k);
     }
 }
 
-// Joins the parts of a row, one wave for each; lane l takes parts l, l + 64, ...
+// Joins the parts of a row, one workgroup for each: the statistics by rescaling, the sorted lists of alternatives by counting larger keys.
+// With as many parts as alternatives, what is below the top-th largest first key is left out beforehand.
 template <class T>
-__global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobsArgs a) {
+__global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobsArgs a) {
+    extern __shared__ u64 lists[];               // parts x top
+    __shared__ u64 found[1024], bound;
+    __shared__ uint32_t count;
+    __shared__ Stats lds[4];
     const int64_t row = block_index();
     if (row >= a.rows) return;
-    const int lane = threadIdx.x;
+    const int tid = threadIdx.x, all = a.parts * a.top;
+    for (int i = tid; i < all; i += 256) lists[i] = a.keys[row * all + i];
+    if (tid == 0) { bound = 1; count = 0; }
     Stats st{kNegInf, 0.0f, 0.0f};
-    for (int p = lane; p < a.parts; p += 64) {
+    for (int p = tid; p < a.parts; p += 256) {
         const Pack<float, 4> q = load<float, 4>(a.stats + (row * a.parts + p) * 4);
         st = join(st, Stats{q.v[0], q.v[1], q.v[2]});
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) st = join(st, Stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)});
-    const bool none = st.s != st.s || st.m == __builtin_inff();
+    if ((tid & 63) == 0) lds[tid >> 6] = st;
+    __syncthreads();
+    st = join(join(lds[0], lds[1]), join(lds[2], lds[3]));
+    const bool none = st.m != st.m || st.m == __builtin_inff();
     const float log_s = __builtin_amdgcn_logf(st.s) * kLn2;
-    if (lane == 0) {
+    if (tid == 0) {
         float xt;
         const int64_t token = token_of<T>(a, row, xt);
         finish_row(a, row, st, log_s, none, xt, token);
     }
-    u64 limit = ~0ull;
-    for (int j = 0; j < a.top; ++j) {
-        u64 best = 0;
-        for (int p = lane; p < a.parts; p += 64) {
-            const u64* k = a.keys + (row * a.parts + p) * a.top;
-            for (int i = 0; i < a.top; ++i) {                       // sorted: the first below the limit is the part's largest
-                if (k[i] < limit) {
-                    best = k[i] > best ? k[i] : best;
-                    break;
-                }
-            }
+    if (!a.top) return;
+    if (a.parts >= a.top) {
+        for (int p = tid; p < a.parts; p += 256) {
+            const u64 k = lists[p * a.top];
+            int rank = 0;
+            for (int i = 0; i < a.parts; ++i) rank += lists[i * a.top] > k;
+            if (rank == a.top - 1 && k) bound = k;
         }
-        limit = lanes_max_key<64>(best);
-        if (lane == 0) write_top(a, row, j, limit, st, log_s, none);
+        __syncthreads();
+    }
+    // at most top lists of top keys each are left
+    for (int i = tid; i < all; i += 256) {
+        const u64 k = lists[i];
+        if (k >= bound) found[atomicAdd(&count, 1u)] = k;
+    }
+    __syncthreads();
+    for (int c = tid; c < (int)count; c += 256) {
+        const u64 k = found[c];
+        int rank = 0;
+        for (int i = 0; i < (int)count; ++i) rank += found[i] > k;
+        if (rank < a.top) write_top(a, row, rank, k, st, log_s, none);
     }
 }
 
 struct LogprobsPlan {
-    int lanes = 64, parts = 1, part_len = 0;
+    int lanes = 64, ept = 32, parts = 1, part_len = 0;
     size_t stats_bytes = 0, bytes = 0;
 };
 
 static bool plan_logprobs(const tae_logprobs_args* p, LogprobsPlan* s) {
     if (p->rows < 1 || p->vocab < 1 || p->vocab > (1 << 21) || p->top < 0 || p->top > 32 || p->top > p->vocab || !dtype_ok(p->dtype)) return false;
     const int V = 16 / (int)dtype_bytes(p->dtype);
-    auto parts_of = [&](int lanes, int ept) {
+    auto parts_of = [&](int lanes, int ept, int spare) {
         s->lanes = lanes;
-        const int most = lanes * ept - V;
+        s->ept = ept;
+        const int most = lanes * ept - spare;    // an unaligned part reaches into one granule more
         s->parts = (int)ceil_div(p->vocab, most);
-        s->part_len = (int)ceil_div(ceil_div(p->vocab, s->parts), V) * V;
+        s->part_len = (int)std::min<int64_t>(most, ceil_div(ceil_div(p->vocab, s->parts), 8) * 8);
         s->parts = (int)ceil_div(p->vocab, s->part_len);
     };
-    if (p->vocab <= 8 * 8 - V) parts_of(8, 8);
-    else if (p->vocab <= 64 * 32 - V || (int64_t)p->rows * p->vocab < (int64_t)512 * 8192) parts_of(64, 32);
-    else parts_of(512, 64);
+    // the fewest lanes that hold a row; long rows in parts, smaller ones where few rows would leave SIMDs empty
+    const int64_t elements = (int64_t)p->rows * p->vocab;
+    if (p->vocab <= 64) parts_of(8, 8, 0);
+    else if (p->vocab <= 512 - V) parts_of(64, 8, V);
+    else if (p->vocab <= 2048 - V || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32, V);
+    else if (p->vocab <= 8192 - V || (elements < (int64_t)512 * 32768 && p->vocab <= (1 << 20))) parts_of(256, 32, V);
+    else parts_of(512, 64, V);
     if (s->parts > 1) {
         s->stats_bytes = (size_t)p->rows * s->parts * 16;
         s->bytes = s->stats_bytes + (size_t)p->rows * s->parts * p->top * 8;
@@ -253,12 +387,15 @@ static bool plan_logprobs(const tae_logprobs_args* p, LogprobsPlan* s) {
 }
 
 template <class T>
-static void launch_logprobs(const LogprobsArgs& a, int lanes, hipStream_t st) {
+static void launch_logprobs(const LogprobsArgs& a, const LogprobsPlan& s, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T);
     const int64_t units = (int64_t)a.rows * a.parts;
-    if (lanes == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 8, 8, 256>), grid_of(ceil_div(units, 32)), dim3(256), 0, st, a);
-    else if (lanes == 64) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 32, 64>), grid_of(units), dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((logprobs_part_kernel<T, 512, 64, 512>), grid_of(units), dim3(512), 0, st, a);
-    if (a.parts > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), grid_of(a.rows), dim3(64), 0, st, a);
+    if (s.lanes == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 8, 8, 1, 256>), grid_of(ceil_div(units, 32)), dim3(256), 0, st, a);
+    else if (s.lanes == 64 && s.ept == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, V, 64>), grid_of(units), dim3(64), 0, st, a);
+    else if (s.lanes == 64) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 32, V, 64>), grid_of(units), dim3(64), 0, st, a);
+    else if (s.lanes == 256) hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 32, V, 256>), grid_of(units), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((logprobs_part_kernel<T, 512, 64, V, 512>), grid_of(units), dim3(512), 0, st, a);
+    if (a.parts > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), grid_of(a.rows), dim3(256), (size_t)a.parts * a.top * 8, st, a);
 }
 
 }  // namespace seq
@@ -293,9 +430,9 @@ int tae_token_logprobs(const tae_logprobs_args* p, void* stream) {
     return guarded([&] {
         hipStream_t st = (hipStream_t)stream;
         switch (p->dtype) {
-            case TAE_DTYPE_F32: launch_logprobs<float>(a, s.lanes, st); break;
-            case TAE_DTYPE_F16: launch_logprobs<f16>(a, s.lanes, st); break;
-            default: launch_logprobs<bf16>(a, s.lanes, st); break;
+            case TAE_DTYPE_F32: launch_logprobs<float>(a, s, st); break;
+            case TAE_DTYPE_F16: launch_logprobs<f16>(a, s, st); break;
+            default: launch_logprobs<bf16>(a, s, st); break;
         }
         return (int)TAE_OK;
     });

@@ -55,15 +55,12 @@ struct Loaded {
 // first exchange leaves positions 0 | 1 (2 | 3) in the two halves of a row and the second 0, 2, 1, 3 in its four quads - 11 instructions
 // instead of 16.  The position whose sum a lane ends up with is `reduced_position`.
 template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
-}
+__device__ __forceinline__ float dpp_add(float v) { return v + dpp<CTRL>(v); }
 template <int CTRL>
 __device__ __forceinline__ float dpp_choose(bool second, float v0, float v1) {
     const float a = dpp_add<CTRL>(v0), b = dpp_add<CTRL>(v1);      // by all lanes, before the choice
     return second ? b : a;
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128;      // quad_perm [1,0,3,2], [2,3,0,1]; row_half_mirror; row_ror:8
 
 template <int P>
 __device__ __forceinline__ int reduced_position(int lane) {
@@ -549,19 +546,19 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int
     const int tid = threadIdx.x, p = tid % P, e = (int)(id % q.groups) * CW + tid / P, E = q.channels;
     const int b0 = (int)(id / q.groups) * each, b1 = min(b0 + each, batch);
     const int k = p * V;                         // V = 4: states are whole groups of four
-    if (e >= E) return;                          // whole groups of lanes that share a channel
-    const bool mine = k < q.n;
+    const int ec = min(e, E - 1);                // lanes without a channel stay for the sums over lanes
+    const bool mine = e < E && k < q.n;
     Pack<float, V> a2{};
     if (mine) a2 = load<float, V>(q.a + (int64_t)e * q.n + k);
-    const float bias = q.dt_bias ? q.dt_bias[e] : 0.0f, dcoef = q.d ? q.d[e] : 0.0f;
+    const float bias = q.dt_bias ? q.dt_bias[ec] : 0.0f, dcoef = q.d ? q.d[ec] : 0.0f;
     for (int b = b0; b < b1; ++b) {
         const int64_t at = ((int64_t)b * E + e) * q.n + k;
         Pack<float, V> h{};
         if (mine && q.state) h = load<float, V>(q.state + at);
         float out = 0.0f;
         if (!q.lengths || q.lengths[b] > 0) {
-            const float x = (float)((const T*)q.x)[b * q.x_b + e];
-            float d = (float)((const T*)q.dt)[b * q.dt_b + e] + bias;
+            const float x = (float)((const T*)q.x)[b * q.x_b + ec];
+            float d = (float)((const T*)q.dt)[b * q.dt_b + ec] + bias;
             if (q.softplus) d = softplus(d);
             if (mine) {
                 const Pack<T, V> bm = load<T, V>((const T*)q.b + b * q.b_b + k), cm = load<T, V>((const T*)q.c + b * q.c_b + k);
@@ -573,9 +570,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int
             }
             out = lanes_sum<P>(out);
             out = __builtin_fmaf(dcoef, x, out);
-            if (q.gate) out *= silu((float)((const T*)q.z)[b * q.z_b + e]);
+            if (q.gate) out *= silu((float)((const T*)q.z)[b * q.z_b + ec]);
         }
-        if (p == 0) ((T*)q.y)[(int64_t)b * E + e] = (T)out;
+        if (p == 0 && e < E) ((T*)q.y)[(int64_t)b * E + e] = (T)out;
         if (mine) store<float, V>(q.state_out + at, h);
     }
 }
