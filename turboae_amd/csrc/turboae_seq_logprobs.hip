@@ -102,16 +102,17 @@ __device__ __forceinline__ uint32_t order_of(u64 k) { return (uint32_t)(k >> 32)
 
 // W lanes (64 or fewer: a share of a wave; more: the workgroup) read a part of a row into registers, EPT elements each, in granules of V.
 //
-// Alternatives: `top` lanes of a wave have a largest element at or above the wave's top-th largest lane maximum, so no element below the
-// largest of these bounds over the waves is among the `top` (the bound is cut to 16 bits, which only lowers it).  What is at or above it, a few
-// dozen elements of a usual row, is collected in LDS in any order and sorted by counting larger keys.  Rows with more than fit (many equal
+// Alternatives: `top` lanes have a largest element at or above the top-th largest lane maximum, so no element below it is among the `top`.
+// The bound is found by bits, by counting lanes that reach it (16 of them: a lower bound does no harm), first in each wave, then among
+// what reaches the largest of these.  Elements at or above it, hardly more than `top` in a usual row, are collected in LDS and sorted by
+// counting larger keys.  Rows with more than fit (many equal
 // values) take the largest one by one.
 template <class T, int W, int EPT, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) {
     constexpr int G = EPT / V, WAVES = W > 64 ? W / 64 : 1, WW = W < 64 ? W : 64, ROOM = W < 64 ? 1 : 128;
     __shared__ float lds_f[WAVES][3];
     __shared__ u64 lds_k[2][WAVES], found[WAVES][ROOM];
-    __shared__ uint32_t lds_u[WAVES], lds_n[WAVES];
+    __shared__ uint32_t lds_u[WAVES], lds_n[WAVES], tops[64], tops_n;
     const int lane = threadIdx.x % W;
     const int64_t unit = block_index() * (THREADS / W) + threadIdx.x / W;
     if (unit >= (int64_t)a.rows * a.parts) return;                  // whole workgroups, or lanes of W < 64, which meet no barrier
@@ -172,25 +173,43 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
     }
     again();
     float m = lanes_join<WW>(mine, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
-    uint32_t bound = 0;
+    uint32_t bound = 0, own = 0;
+    // the largest 16-bit prefix that `top` of the wave's 64 values reach
+    auto reached = [&](uint32_t v) {
+        uint32_t prefix = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t with = prefix | 1u << bit;
+            if (__popcll(__ballot(v >= with)) >= a.top) prefix = with;
+        }
+        return prefix;
+    };
     if constexpr (W >= 64) {
         if (a.top) {
-            // the largest 16-bit prefix that `top` lane maxima of this wave reach
-            const uint32_t own = lo - skew + lane * V < hi ? order_of(key_of(mine, 0)) : 0u;
-#pragma unroll
-            for (int bit = 31; bit >= 16; --bit) {
-                const uint32_t with = bound | 1u << bit;
-                if (__popcll(__ballot(own >= with)) >= a.top) bound = with;
-            }
+            own = lo - skew + lane * V < hi ? order_of(key_of(mine, 0)) : 0u;
+            bound = reached(own);
         }
     }
     if constexpr (W > 64) {
         if ((threadIdx.x & 63) == 0) { lds_f[wave][0] = m; lds_u[wave] = bound; }
+        if (threadIdx.x == 0) tops_n = 0;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) { m = __builtin_elementwise_maximum(m, lds_f[i][0]); bound = max(bound, lds_u[i]); }
     }
-    // e^(x - m) = 2^(x log2 e - m log2 e); -inf (and what is far below m) is taken at 2^-1000 = 0, so that 0 times its distance is 0
+    if constexpr (W > 64) {
+        // lane maxima at or above that bound, of the whole workgroup: where they fit one wave, they give a closer one below
+        const u64 set = __ballot(a.top && own >= bound);
+        if (set) {
+            uint32_t first = 0;
+            if ((threadIdx.x & 63) == 0) first = atomicAdd(&tops_n, (uint32_t)__popcll(set));
+            first = __builtin_amdgcn_readfirstlane(first);
+            const uint32_t slot = first + __builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
+            if (a.top && own >= bound && slot < 64) tops[slot] = own;
+        }
+    }
+    // e^(x - m) = 2^((x - m) log2 e), the difference first: one fused instruction less would lose it next to a maximum like the type's lowest
+    // value; -inf (and what is far below m) is taken at 2^-1000 = 0, so that 0 times its distance is 0
     const float base = m == kNegInf ? 0.0f : m;
     float s = 0.0f, t = 0.0f;
 #pragma unroll
@@ -229,6 +248,9 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
         else a.keys[unit * a.top + j] = k;
     };
     if constexpr (W >= 64) {
+        if constexpr (W > 64) {
+            if (tops_n <= 64) bound = max(bound, reached((threadIdx.x & 63) < tops_n ? tops[threadIdx.x & 63] : 0u));
+        }
         // each wave's own list, filled in the order of granules and lanes; granules without a candidate cost one comparison
         const float least = bound ? key_value((u64)bound << 32) : kNegInf;
         uint32_t n = 0;
@@ -246,6 +268,7 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
                 n += __popcll(set);
             }
         }
+        if ((threadIdx.x & 63) < 8 && n + (threadIdx.x & 63) < ROOM) found[wave][n + (threadIdx.x & 63)] = 0;      // whole groups of eight
         bool fits = n <= ROOM;
         uint32_t total = n;
         if constexpr (W > 64) {
@@ -268,7 +291,10 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
                 int rank = 0;
                 for (int u = 0; u < WAVES; ++u) {
                     const int count = W > 64 ? (int)lds_n[u] : (int)n;
-                    for (int i = 0; i < count; ++i) rank += found[u][i] > k;
+                    for (int i = 0; i < count; i += 8) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) rank += found[u][i + j] > k;
+                    }
                 }
                 if (rank < a.top) put(rank, k);
             }
@@ -348,10 +374,15 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobsArgs a) {
         if (k >= bound) found[atomicAdd(&count, 1u)] = k;
     }
     __syncthreads();
+    if (tid < 8 && count + tid < 1024) found[count + tid] = 0;      // whole groups of eight
+    __syncthreads();
     for (int c = tid; c < (int)count; c += 256) {
         const u64 k = found[c];
         int rank = 0;
-        for (int i = 0; i < (int)count; ++i) rank += found[i] > k;
+        for (int i = 0; i < (int)count; i += 8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rank += found[i + j] > k;
+        }
         if (rank < a.top) write_top(a, row, rank, k, st, log_s, none);
     }
 }
@@ -361,24 +392,26 @@ struct LogprobsPlan {
     size_t stats_bytes = 0, bytes = 0;
 };
 
-static bool plan_logprobs(const tae_logprobs_args* p, LogprobsPlan* s) {
+// aligned_rows: every row starts on a 16-byte boundary (an unaligned part reaches into one granule more)
+static bool plan_logprobs(const tae_logprobs_args* p, bool aligned_rows, LogprobsPlan* s) {
     if (p->rows < 1 || p->vocab < 1 || p->vocab > (1 << 21) || p->top < 0 || p->top > 32 || p->top > p->vocab || !dtype_ok(p->dtype)) return false;
     const int V = 16 / (int)dtype_bytes(p->dtype);
-    auto parts_of = [&](int lanes, int ept, int spare) {
+    const int spare = aligned_rows ? 0 : V;
+    auto parts_of = [&](int lanes, int ept) {
         s->lanes = lanes;
         s->ept = ept;
-        const int most = lanes * ept - spare;    // an unaligned part reaches into one granule more
+        const int most = lanes * ept - spare;
         s->parts = (int)ceil_div(p->vocab, most);
         s->part_len = (int)std::min<int64_t>(most, ceil_div(ceil_div(p->vocab, s->parts), 8) * 8);
         s->parts = (int)ceil_div(p->vocab, s->part_len);
     };
     // the fewest lanes that hold a row; long rows in parts, smaller ones where few rows would leave SIMDs empty
     const int64_t elements = (int64_t)p->rows * p->vocab;
-    if (p->vocab <= 64) parts_of(8, 8, 0);
-    else if (p->vocab <= 512 - V) parts_of(64, 8, V);
-    else if (p->vocab <= 2048 - V || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32, V);
-    else if (p->vocab <= 8192 - V || (elements < (int64_t)512 * 32768 && p->vocab <= (1 << 20))) parts_of(256, 32, V);
-    else parts_of(512, 64, V);
+    if (p->vocab <= 64) parts_of(8, 8);
+    else if (p->vocab <= 512 - spare) parts_of(64, 8);
+    else if (p->vocab <= 2048 - spare || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32);
+    else if (p->vocab <= 8192 - spare || (elements < (int64_t)1024 * 8192 && p->vocab <= (1 << 20))) parts_of(256, 32);
+    else parts_of(256, 64);
     if (s->parts > 1) {
         s->stats_bytes = (size_t)p->rows * s->parts * 16;
         s->bytes = s->stats_bytes + (size_t)p->rows * s->parts * p->top * 8;
@@ -393,8 +426,8 @@ static void launch_logprobs(const LogprobsArgs& a, const LogprobsPlan& s, hipStr
     if (s.lanes == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 8, 8, 1, 256>), grid_of(ceil_div(units, 32)), dim3(256), 0, st, a);
     else if (s.lanes == 64 && s.ept == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, V, 64>), grid_of(units), dim3(64), 0, st, a);
     else if (s.lanes == 64) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 32, V, 64>), grid_of(units), dim3(64), 0, st, a);
-    else if (s.lanes == 256) hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 32, V, 256>), grid_of(units), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((logprobs_part_kernel<T, 512, 64, V, 512>), grid_of(units), dim3(512), 0, st, a);
+    else if (s.ept == 32) hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 32, V, 256>), grid_of(units), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 64, V, 256>), grid_of(units), dim3(256), 0, st, a);
     if (a.parts > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), grid_of(a.rows), dim3(256), (size_t)a.parts * a.top * 8, st, a);
 }
 
@@ -405,9 +438,9 @@ extern "C" {
 
 size_t tae_token_logprobs_workspace(const tae_logprobs_args* p) {
     using namespace tae::seq;
-    LogprobsPlan s;
-    if (!p || p->struct_size != (int32_t)sizeof(tae_logprobs_args) || !plan_logprobs(p, &s)) return 0;
-    return s.bytes;
+    LogprobsPlan s, u;
+    if (!p || p->struct_size != (int32_t)sizeof(tae_logprobs_args) || !plan_logprobs(p, true, &s) || !plan_logprobs(p, false, &u)) return 0;
+    return std::max(s.bytes, u.bytes);
 }
 
 int tae_token_logprobs(const tae_logprobs_args* p, void* stream) {
@@ -422,7 +455,8 @@ int tae_token_logprobs(const tae_logprobs_args* p, void* stream) {
     if (p->top && (!p->top_ids || !p->top_logp)) return fail_msg(TAE_EINVAL, "token_logprobs: top needs top_ids and top_logp");
     if (!aligned(p->logits, dtype_bytes(p->dtype)) || !aligned(p->tokens, p->token_bytes)) return fail_msg(TAE_EINVAL, "token_logprobs: a pointer is not aligned to its elements");
     LogprobsPlan s;
-    if (!plan_logprobs(p, &s)) return fail_msg(TAE_EINVAL, "token_logprobs: bad sizes");
+    const bool rows16 = aligned(p->logits, 16) && p->logits_row * (int64_t)dtype_bytes(p->dtype) % 16 == 0;
+    if (!plan_logprobs(p, rows16, &s)) return fail_msg(TAE_EINVAL, "token_logprobs: bad sizes");
     if (s.bytes && (!p->workspace || p->workspace_bytes < s.bytes || !aligned(p->workspace, 16)))
         return fail_msg(TAE_EINVAL, "token_logprobs: the workspace is missing, misaligned or smaller than tae_token_logprobs_workspace");
     LogprobsArgs a{p->logits, p->tokens, p->logp, p->entropy, p->top_logp, p->top_ids, s.bytes ? (float*)p->workspace : nullptr,
