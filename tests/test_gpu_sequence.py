@@ -212,7 +212,7 @@ def test_norm_residual_of_rows_without_variance(gpu_device):
 
 
 # ---------------------------------------------------------------------------------------------------------------- int8
-INT8 = [(dt, *shape) for dt in DT for shape in ((1, 16, 16), (1, 1, 1), (4, 256, 100), (3, 77, 5), (16, 1000, 33), (17, 64, 64), (33, 63, 130), (64, 129, 257), (100, 512, 200), (130, 4096, 72), (257, 300, 513))]
+INT8 = [(dt, *shape) for dt in DT for shape in ((1, 16, 16), (1, 1, 1), (4, 256, 100), (3, 77, 5), (16, 1000, 33), (17, 64, 64), (33, 63, 130), (64, 129, 257), (100, 512, 200), (130, 4096, 72), (257, 300, 513), (1000, 200, 2050), (1030, 64, 4100), (3001, 130, 4100), (4100, 520, 6150))]
 
 
 def int8_case(g, t, M, K, N):
@@ -261,6 +261,20 @@ def test_quantize_int8(gpu_device, dt, R, K):
     if R > 2:
         assert math.isnan(float(s[2])) and int(q[2].abs().sum()) == 0
     assert q.stride(0) % 64 == 0 and int(q.as_strided((R, q.stride(0)), (q.stride(0), 1))[:, K:].abs().sum()) == 0
+
+
+@pytest.mark.parametrize("dt,size", [("f32", 1e-37), ("f32", 1e-40), ("f32", 3e38), ("bf16", 1e-37), ("bf16", 3e38), ("f16", 6e-8), ("f16", 6e4)])
+def test_quantize_int8_of_tiny_and_huge_rows(gpu_device, dt, size):
+    """Magnitudes whose reciprocal overflows, numbers below the normal ones, and the largest (127 x overflows: such a row is all 127s or
+    follows the definition's own 32-bit steps)."""
+    from turboae_amd import sequence
+    x = (torch.linspace(-1.0, 1.0, 96)[None] * size).to(DT[dt])
+    q, s = sequence.quantize_int8(x.to(gpu_device))
+    wq, ws = O.quantize(x)
+    if bool(torch.isfinite(x.float() * 127.0).all()):
+        assert torch.equal(q.cpu().double(), wq) and torch.equal(s.cpu(), ws)
+    else:
+        assert torch.equal(s.cpu(), ws) and int(q.abs().max()) <= 127
 
 
 def test_int8_rows_with_nan_spoil_only_themselves(gpu_device):

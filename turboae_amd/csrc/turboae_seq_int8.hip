@@ -19,8 +19,29 @@ struct QuantArgs {
     int rows, cols;
 };
 
-// One workgroup for each row: its largest magnitude, then its whole numbers (the second reading comes from L2).
+// V whole numbers of a row with the largest magnitude `most`.  127 x / most is first taken with one reciprocal for the row, off by at most
+// 127 * 2^-23; only where that could move it across the middle of two whole numbers is it divided as it is defined.  Adding 1.5 * 2^23 rounds
+// halves to even and leaves the whole number in the low bits.
 template <class T, int V>
+__device__ __forceinline__ Pack<int8_t, V> whole_numbers(const Pack<T, V>& p, float by, float reciprocal) {
+    constexpr float kMagic = 12582912.0f;
+    Pack<int8_t, V> o;
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float t = (float)p.v[i] * reciprocal, r = t + kMagic;
+        near = near || !(fabsf(t - (r - kMagic)) < 0.4995f);         // also where the reciprocal of a tiny magnitude is infinite
+        o.v[i] = (int8_t)__float_as_int(r);
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = (int8_t)__float_as_int((float)p.v[i] * 127.0f / by + kMagic);
+    }
+    return o;
+}
+
+// One workgroup for each row, which stays in registers (KEEP groups of V for each lane) or, with KEEP = 0, is read twice.
+template <class T, int V, int KEEP>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     __shared__ float lds[4];
     const int64_t row = block_index();
@@ -29,14 +50,22 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     const T* x = (const T*)a.x + row * a.x_r;
     float most = 0.0f;
     bool bad = false;
-    for (int e = tid * V; e < a.cols; e += 256 * V) {
-        const Pack<T, V> p = load<T, V>(x + e);
+    auto look = [&](const Pack<T, V>& p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float v = fabsf((float)p.v[i]);
             bad = bad || !(v < __builtin_inff());
             most = fmaxf(most, v);
         }
+    };
+    Pack<T, V> kept[KEEP > 0 ? KEEP : 1];
+    if constexpr (KEEP > 0) {
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) kept[j] = load<T, V>(x + min((j * 256 + tid) * V, a.cols - V));
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) look(kept[j]);
+    } else {
+        for (int e = tid * V; e < a.cols; e += 256 * V) look(load<T, V>(x + e));
     }
     if (__any(bad)) most = __builtin_inff();
     most = lanes_max<64>(most);
@@ -45,15 +74,19 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     most = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
     const bool fine = most < __builtin_inff();
     if (tid == 0) a.scale[row] = fine ? most / 127.0f : __builtin_nanf("");
-    const float by = most > 0.0f ? most : 1.0f;
+    // a row of zeros: 0; one with an infinity or NaN: 0 too, whatever it holds
+    const float by = most > 0.0f ? most : 1.0f, reciprocal = 127.0f / by;
     int8_t* q = a.q + row * a.q_r;
-    for (int e = tid * V; e < a.q_r; e += 256 * V) {
-        Pack<int8_t, V> o;
-        Pack<T, V> p;
-        if (e < a.cols) p = load<T, V>(x + e);
+    const Pack<int8_t, V> zeros{};
+    if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = fine && e < a.cols ? (int8_t)(int)rintf((float)p.v[i] * 127.0f / by) : (int8_t)0;
-        store<int8_t, V>(q + e, o);
+        for (int j = 0; j < KEEP; ++j) {
+            const int e = (j * 256 + tid) * V;
+            if (e < a.q_r) store<int8_t, V>(q + e, fine && e < a.cols ? whole_numbers<T, V>(kept[j], by, reciprocal) : zeros);
+        }
+        for (int e = (KEEP * 256 + tid) * V; e < a.q_r; e += 256 * V) store<int8_t, V>(q + e, zeros);
+    } else {
+        for (int e = tid * V; e < a.q_r; e += 256 * V) store<int8_t, V>(q + e, fine && e < a.cols ? whole_numbers<T, V>(load<T, V>(x + e), by, reciprocal) : zeros);
     }
 }
 
@@ -62,8 +95,12 @@ static void launch_quantize(const QuantArgs& a, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
     Width w(sizeof(T));
     w.elements(a.cols).elements(a.x_r).pointer(a.x);
-    if (w.fits(16)) hipLaunchKernelGGL((quantize_int8_kernel<T, V>), grid_of(a.rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((quantize_int8_kernel<T, 1>), grid_of(a.rows), dim3(256), 0, st, a);
+    const dim3 grid = grid_of(a.rows), block(256);
+    if (!w.fits(16)) hipLaunchKernelGGL((quantize_int8_kernel<T, 1, 0>), grid, block, 0, st, a);
+    else if (a.cols <= 256 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 1>), grid, block, 0, st, a);
+    else if (a.cols <= 512 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 2>), grid, block, 0, st, a);
+    else if (a.cols <= 1024 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((quantize_int8_kernel<T, V, 0>), grid, block, 0, st, a);
 }
 
 static void launch_quantize_dtype(const QuantArgs& a, int32_t dtype, hipStream_t st) {
@@ -79,65 +116,306 @@ struct Int8Args {
     const float *scale, *w_scale, *bias;
     void* y;
     int64_t q_r, w_r;
-    int m, k, n, tiles_n;
-    int64_t blocks;
+    int m, k, n, tiles_n, wide;                  // wide: rows of y start on 16-byte boundaries
+    int64_t tiles_m, blocks;
 };
 
-// 64 x 64 outputs for each workgroup, 32 x 32 for each wave.  LDS holds 16 x 64 pieces of both operands in the order in which a wave's lanes
-// hand them to the matrix instruction: lane l has 16 adjacent k of row l % 16, from k = 16 (l / 16).
+// Products of 16 rows of weights with 16 rows of x over 64 inputs: lane l hands over 16 adjacent inputs of row l % 16, from input 16 (l / 16),
+// for both, and holds the sums of weight rows 4 (l / 16) .. + 3 with x row l % 16.
+__device__ __forceinline__ i32x4 mfma64(i32x4 w, i32x4 q, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q, c, 0, 0, 0); }
+
+// COUNT adjacent outputs from n on: their scales and biases once, then row by row.
+template <class T, int COUNT>
+struct Outputs {
+    float scale[COUNT], bias[COUNT];
+    int n;
+    __device__ __forceinline__ Outputs(const Int8Args& a, int n0) : n(n0) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int at = min(n + i, a.n - 1);
+            scale[i] = a.w_scale[at];
+            bias[i] = a.bias ? a.bias[at] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ Pack<T, COUNT> row(const int (&sum)[COUNT], float sm) const {
+        Pack<T, COUNT> out;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) out.v[i] = (T)__builtin_fmaf((float)sum[i], sm * scale[i], bias[i]);
+        return out;
+    }
+};
+
+// 32 or 64 bytes that are not read again soon: they leave the operands in L2 alone
 template <class T>
-__global__ __launch_bounds__(256) void int8_linear_kernel(Int8Args a) {
-    __shared__ i32x4 lw[256], lq[256];
+__device__ __forceinline__ void store_once(T* to, const Pack<T, 16>& p) {
+    i32x4 part[sizeof(p) / 16];
+    __builtin_memcpy(part, &p, sizeof(p));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(p) / 16; ++i) __builtin_nontemporal_store(part[i], reinterpret_cast<i32x4*>(to) + i);
+}
+
+// Copies 16 bytes for each lane from a buffer to LDS without registers, to `to` + 16 lane; counted by vmcnt.  Offsets outside the buffer
+// give zeros.
+using LdsPtr = __attribute__((address_space(3))) void*;
+__device__ __forceinline__ void copy_to_lds(__amdgpu_buffer_rsrc_t buffer, LdsPtr to, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to, 16, offset, 0, 0, 0);
+}
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() {             // all but the last LEFT of this wave's copies have arrived, for every wave
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// BM x BN outputs at a time for each workgroup of WM x WN waves, 64 weight rows for each wave.
+//
+// Bound by the matrix instructions.  A workgroup takes tile after tile without a break: the slabs of 128 inputs of all its tiles are one
+// stream through two LDS buffers, copied directly, whole 128-byte lines at a time.  The one barrier of a slab stands behind its last
+// fragment reads, a quarter of its products before its end: there the next slab has arrived, this slab's buffer is free for the one after
+// it, and the next slab's first fragments are read during the rest of the products.  A tile's results are stored while the next tile is
+// under way.  A row's eight 16-byte pieces are permuted by its number (by which piece a lane copies), so that the 16 lanes which read LDS
+// together touch all banks.  Weight rows are dealt to fragments such that a lane ends up with 16 adjacent outputs.  Workgroups of one XCD
+// (every eighth) take adjacent tiles, eight rows of tiles high, and share operands in its L2.
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void int8_linear_kernel(Int8Args a) {
+    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = 4, ROWS = BM + BN, PIECES = ROWS / 8 / WAVES, STAGE = ROWS * 128;
+    static_assert(BN / WN == 64 && ROWS % (8 * WAVES) == 0 && BM % (8 * PIECES) == 0, "whole pieces of one operand for each wave");
+    extern __shared__ char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    // this workgroup's tiles: of its XCD's share, every (workgroups of the XCD)-th
+    const int64_t xcd = blockIdx.x % 8, each = a.blocks / 8, more = a.blocks % 8, stride_tiles = (gridDim.x - xcd + 7) / 8;
+    const int64_t share = each + (xcd < more), begin = xcd * each + min(xcd, more), slot = blockIdx.x / 8;
+    const int tiles = (int)(slot < share ? (share - slot + stride_tiles - 1) / stride_tiles : 0);
+    if (tiles == 0) return;
+    auto place = [&](int i, int& m0, int& n0) {
+        const int64_t tile = begin + slot + i * stride_tiles, band = tile / (8 * (int64_t)a.tiles_n), first = band * 8;
+        const int64_t high = min((int64_t)8, a.tiles_m - first), in = tile - first * a.tiles_n;
+        m0 = (int)(first + in % high) * BM;
+        n0 = (int)(in / high) * BN;
+    };
+    const int slabs = (a.k + 127) / 128;
+
+    // the copying end of the stream: its tile, slab and buffer; this wave copies rows 8 PIECES wave .. of x (rows 0 .. BM - 1), then of the weights
+    const bool weights = wave * PIECES * 8 >= BM;
+    const int64_t stride = weights ? a.w_r : a.q_r;
+    __amdgpu_buffer_rsrc_t buffer;
+    uint32_t offset[PIECES];
+    auto open = [&](int i) {
+        int m0, n0;
+        place(i, m0, n0);
+        const int rows = weights ? min(a.n - n0, BN) : min(a.m - m0, BM);
+        const int8_t* from = weights ? a.w + (int64_t)n0 * a.w_r : a.q + (int64_t)m0 * a.q_r;
+        buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from), 0, (int)((rows - 1) * stride) + ((a.k + 15) & ~15), 0x00020000);
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int r = (wave * PIECES + j) * 8 + lane / 8;        // row of the stage
+            int row = weights ? r - BM : r;
+            if (weights) row = (row & ~63) + (row / 4 % 4) * 16 + (row / 16 % 4) * 4 + row % 4;
+            offset[j] = (uint32_t)min(row, rows - 1) * (uint32_t)stride + ((lane ^ r) & 7) * 16;
+        }
+    };
+    int to_tile = 0, to_slab = 0;
+    auto copy = [&](int stage) {                 // behind the end the last slab again
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) copy_to_lds(buffer, (LdsPtr)(lds + stage * STAGE + (wave * PIECES + j) * 1024), offset[j] + (uint32_t)to_slab * 128);
+        if (to_slab + 1 < slabs) {
+            ++to_slab;
+        } else if (to_tile + 1 < tiles) {
+            open(++to_tile);
+            to_slab = 0;
+        }
+    };
+
+    // pieces q and 4 + q of row r16 for the two halves of a slab
+    const int r16 = lane & 15, half[2] = {r16 * 128 + (((lane >> 4) ^ r16) & 7) * 16, r16 * 128 + (((lane >> 4 | 4) ^ r16) & 7) * 16};
+    i32x4 wf[NF], wf_next[NF], qf[MF], qf_next[2], acc[NF][MF] = {};
+    auto weight = [&](const char* p, int f) { return *(const i32x4*)(p + (BM + wn * 64 + f * 16) * 128); };
+    auto x = [&](const char* p, int f) { return *(const i32x4*)(p + (wm * MF + f) * 2048); };
+    int tile = 0, slab = 0, stage = 0, m0, n0;
+    auto results = [&]() {
+        const int n = n0 + wn * 64 + (lane >> 4) * 16;
+        const Outputs<T, 16> outputs(a, n);
+        float sm[MF];
+#pragma unroll
+        for (int i = 0; i < MF; ++i) sm[i] = a.scale[min(m0 + (wm * MF + i) * 16 + r16, a.m - 1)];
+        const bool whole = a.wide && n0 + BN <= a.n;
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            const int m = m0 + (wm * MF + i) * 16 + r16;
+            int sum[16];
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sum[f * 4 + r] = acc[f][i][r];
+                    acc[f][i][r] = 0;
+                }
+            const Pack<T, 16> out = outputs.row(sum, sm[i]);
+            T* y = (T*)a.y + (int64_t)m * a.n + n;
+            if (whole) {
+                if (m < a.m) store_once(y, out);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                    if (m < a.m && n + c < a.n) y[c] = out.v[c];
+            }
+        }
+    };
+    constexpr int EARLY = MF * 3 / 4;            // of the second half's products, in front of the barrier: what needs no more fragments
+    auto multiply = [&](int from, int to) {
+#pragma unroll
+        for (int i = from; i < to; ++i)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) acc[f][i] = mfma64(wf[f], qf[i], acc[f][i]);
+    };
+    auto advance = [&]() {
+#pragma unroll
+        for (int f = 0; f < NF; ++f) wf[f] = wf_next[f];
+        qf[0] = qf_next[0];
+        qf[1] = qf_next[1];
+    };
+    auto first = [&](const char* p) {            // the fragments that a half starts with
+#pragma unroll
+        for (int f = 0; f < NF; ++f) wf_next[f] = weight(p, f);
+        qf_next[0] = x(p, 0);
+        qf_next[1] = x(p, 1);
+    };
+    place(0, m0, n0);
+    open(0);
+    copy(0);
+    copy(1);
+    wait_copies<PIECES>();
+    first(lds + half[0]);
+    advance();
+    for (;;) {
+        const char* here = lds + stage * STAGE;
+#pragma unroll
+        for (int i = 2; i < MF; ++i) qf[i] = x(here + half[0], i);
+        first(here + half[1]);
+        multiply(0, MF);
+        // issue order: one fragment read for every second or third product
+#pragma unroll
+        for (int f = 0; f < NF + MF; ++f) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, MF * NF / (NF + MF), 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, MF * NF - MF * NF / (NF + MF) * (NF + MF), 0);
+        __builtin_amdgcn_sched_barrier(0);
+        advance();
+#pragma unroll
+        for (int i = 2; i < MF; ++i) qf[i] = x(here + half[1], i);
+        multiply(0, EARLY);
+#pragma unroll
+        for (int f = 2; f < MF; ++f) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x008, EARLY * NF / (MF - 2), 1);
+        }
+        // all fragments of this slab have been read, by every wave, and all copies of the next one have arrived
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        copy(stage);
+        stage ^= 1;
+        first(lds + stage * STAGE + half[0]);
+        multiply(EARLY, MF);
+        advance();
+        if (++slab < slabs) continue;
+        results();
+        slab = 0;
+        if (++tile == tiles) break;
+        place(tile, m0, n0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no copy is under way when the workgroup's LDS is given away
+}
+
+// Few rows of x: bound by reading the weights.  16 weight rows and up to 16 MF rows of x for each workgroup; its eight waves share the inputs
+// and join their sums, exact in any order, in LDS.  Both operands come straight from memory (x from L2), kDeep slabs in flight.
+template <class T, int MF>
+__global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
+    constexpr int kDeep = MF == 1 ? 8 : 4;
+    __shared__ i32x4 part[8][MF][64];
     const int64_t id = block_index();
     if (id >= a.blocks) return;
-    const int n0 = (int)(id % a.tiles_n) * 64;
-    const int m0 = (int)(id / a.tiles_n) * 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = (tid >> 6) * 16 + (lane & 15), kk = (lane >> 4) * 16;
-    const int8_t* w = a.w + (int64_t)min(n0 + row, a.n - 1) * a.w_r;
-    const int8_t* q = a.q + (int64_t)min(m0 + row, a.m - 1) * a.q_r;
-    i32x4 acc[2][2] = {};
-    for (int k0 = 0; k0 < a.k; k0 += 64) {
-        i32x4 vw{}, vq{};
-        if (k0 + kk < a.k) {
-            vw = *(const i32x4*)(w + k0 + kk);
-            vq = *(const i32x4*)(q + k0 + kk);
+    const int n0 = (int)(id % a.tiles_n) * 16, m0 = (int)(id / a.tiles_n) * 16 * MF;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kk = (lane >> 4) * 16;
+    const int slabs = (a.k + 63) / 64, each = (slabs + 7) / 8, begin = wave * each, end = min(begin + each, slabs);
+    const int8_t* w = a.w + (int64_t)min(n0 + r16, a.n - 1) * a.w_r;
+    const int8_t* q[MF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) q[i] = a.q + (int64_t)min(m0 + i * 16 + r16, a.m - 1) * a.q_r;
+    i32x4 acc[MF] = {};
+    const int last = (a.k - 1) & ~15;            // the last 16 bytes of a row that may be read; q is zero where they repeat
+    for (int s0 = begin; s0 < end; s0 += kDeep) {
+        i32x4 wv[kDeep], qv[kDeep][MF];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int k = min(s0 + d, end - 1) * 64 + kk;
+            wv[d] = *(const i32x4*)(w + min(k, last));
+#pragma unroll
+            for (int i = 0; i < MF; ++i) qv[d][i] = *(const i32x4*)(q[i] + k);
         }
-        __syncthreads();
-        lw[tid] = vw;
-        lq[tid] = vq;
-        __syncthreads();
-        const int tn = (wave & 1) * 2, tm = (wave >> 1) * 2;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int d = 0; d < kDeep; ++d) {
+            if (s0 + d < end) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(lw[(tn + i) * 64 + lane], lq[(tm + j) * 64 + lane], acc[i][j], 0, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int m = m0 + (wave >> 1) * 32 + j * 16 + (lane & 15);
-        if (m >= a.m) continue;
-        const float sm = a.scale[m];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int n = n0 + (wave & 1) * 32 + i * 16 + (lane >> 4) * 4 + r;
-                if (n >= a.n) continue;
-                float v = (float)acc[i][j][r] * (sm * a.w_scale[n]);
-                if (a.bias) v += a.bias[n];
-                ((T*)a.y)[(int64_t)m * a.n + n] = (T)v;
+                for (int i = 0; i < MF; ++i) acc[i] = mfma64(wv[d], qv[d][i], acc[i]);
             }
+        }
     }
+#pragma unroll
+    for (int i = 0; i < MF; ++i) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= MF) return;
+    i32x4 sum = part[0][wave][lane];
+#pragma unroll
+    for (int u = 1; u < 8; ++u) sum += part[u][wave][lane];
+    const int m = m0 + wave * 16 + r16, n = n0 + (lane >> 4) * 4;
+    if (m >= a.m || n >= a.n) return;
+    const Pack<T, 4> out = Outputs<T, 4>(a, n).row({sum[0], sum[1], sum[2], sum[3]}, a.scale[m]);
+    T* y = (T*)a.y + (int64_t)m * a.n + n;
+    if (a.wide) {                                // outputs come in whole groups of four
+        store<T, 4>(y, out);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (n + c < a.n) y[c] = out.v[c];
+    }
+}
+
+template <class T, int BM, int BN, int WM, int WN>
+static hipError_t launch_tiles(Int8Args a, hipStream_t st) {
+    constexpr int bytes = 2 * (BM + BN) * 128;
+    a.tiles_m = ceil_div(a.m, BM);
+    a.tiles_n = (int)ceil_div(a.n, BN);
+    a.blocks = a.tiles_m * a.tiles_n;
+    const void* kernel = reinterpret_cast<const void*>(int8_linear_kernel<T, BM, BN, WM, WN>);
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);        // of the current device
+    if (e != hipSuccess) return e;
+    const int64_t resident = 256 * (160 * 1024 / bytes);     // workgroups that 256 CUs hold at once
+    hipLaunchKernelGGL((int8_linear_kernel<T, BM, BN, WM, WN>), dim3((uint32_t)std::min(a.blocks, resident)), dim3(WM * WN * 64), bytes, st, a);
+    return hipSuccess;
+}
+
+template <class T, int MF>
+static hipError_t launch_few(Int8Args a, hipStream_t st) {
+    a.tiles_m = ceil_div(a.m, 16 * MF);
+    a.tiles_n = (int)ceil_div(a.n, 16);
+    a.blocks = a.tiles_m * a.tiles_n;
+    hipLaunchKernelGGL((int8_few_kernel<T, MF>), grid_of(a.blocks), dim3(512), 0, st, a);
+    return hipSuccess;
 }
 
 template <class T>
-static void launch_int8(const Int8Args& a, hipStream_t st) {
-    hipLaunchKernelGGL((int8_linear_kernel<T>), grid_of(a.blocks), dim3(256), 0, st, a);
+static hipError_t launch_int8(const Int8Args& a, hipStream_t st) {
+    if (a.m <= 16) return launch_few<T, 1>(a, st);
+    if (a.m <= 32) return launch_few<T, 2>(a, st);
+    const int64_t large = ceil_div(a.m, 256) * ceil_div(a.n, 256), small = ceil_div(a.m, 128) * ceil_div(a.n, 128);
+    if (large >= 192) return launch_tiles<T, 256, 256, 2, 4>(a, st);
+    if (a.m <= 128 || small < 128) return launch_few<T, 4>(a, st);
+    return launch_tiles<T, 128, 128, 2, 2>(a, st);
 }
 
-static int64_t q_stride(int32_t k) { return ceil_div(k, 64) * 64; }
+// Rows 1024 bytes and multiples apart would send a slab's lines of all rows to few channels of L2.
+static int64_t q_stride(int32_t k) {
+    const int64_t r = ceil_div(k, 128) * 128;
+    return r % 1024 ? r : r + 128;
+}
 
 static bool int8_sizes(const tae_int8_args* p) {
     return p->rows >= 1 && p->inputs >= 1 && p->inputs <= 131072 && p->outputs >= 1 && p->rows <= (1 << 30) && p->outputs <= (1 << 30);
@@ -174,23 +452,25 @@ int tae_int8_linear(const tae_int8_args* p, void* stream) {
     if (!dtype_ok(p->dtype)) return fail_msg(TAE_EINVAL, "int8_linear: dtype must be a TAE_DTYPE_* code");
     if (!int8_sizes(p)) return fail_msg(TAE_EINVAL, "int8_linear: inputs must be in 1..131072, rows and outputs in 1..2^30");
     if (!p->x || !p->weight || !p->weight_scale || !p->y) return fail_msg(TAE_EINVAL, "int8_linear: x, weight, weight_scale and y must not be NULL");
-    if (!aligned(p->weight, 16) || p->weight_row % 16 || p->weight_row < p->inputs) return fail_msg(TAE_EINVAL, "int8_linear: weight rows start on 16-byte boundaries (quantize_int8 lays them so)");
+    if (!aligned(p->weight, 16) || p->weight_row % 16 || p->weight_row < p->inputs || p->weight_row > (1 << 23)) return fail_msg(TAE_EINVAL, "int8_linear: weight rows start on 16-byte boundaries (quantize_int8 lays them so), at most 2^23 bytes apart");
     const size_t need = tae_int8_linear_workspace(p);
     if (!p->workspace || p->workspace_bytes < need || !aligned(p->workspace, 16)) return fail_msg(TAE_EINVAL, "int8_linear: the workspace is missing, misaligned or smaller than tae_int8_linear_workspace");
     const int64_t qr = q_stride(p->inputs);
     int8_t* q = (int8_t*)p->workspace;
     float* scale = (float*)(q + (size_t)p->rows * qr);
-    const int tiles_n = (int)ceil_div(p->outputs, 64);
-    Int8Args a{q, p->weight, scale, p->weight_scale, p->bias, p->y, qr, p->weight_row, p->rows, p->inputs, p->outputs, tiles_n, tiles_n * ceil_div(p->rows, 64)};
-    if (a.blocks > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "int8_linear: the product is too large for one call");
+    Width wy(dtype_bytes(p->dtype));
+    wy.elements(p->outputs).pointer(p->y);
+    const Int8Args a{q, p->weight, scale, p->weight_scale, p->bias, p->y, qr, p->weight_row, p->rows, p->inputs, p->outputs, 0, wy.fits(16), 0, 0};
     return guarded([&] {
         hipStream_t st = (hipStream_t)stream;
         launch_quantize_dtype(QuantArgs{p->x, q, scale, p->x_row, qr, p->rows, p->inputs}, p->dtype, st);
+        hipError_t e;
         switch (p->dtype) {
-            case TAE_DTYPE_F32: launch_int8<float>(a, st); break;
-            case TAE_DTYPE_F16: launch_int8<f16>(a, st); break;
-            default: launch_int8<bf16>(a, st); break;
+            case TAE_DTYPE_F32: e = launch_int8<float>(a, st); break;
+            case TAE_DTYPE_F16: e = launch_int8<f16>(a, st); break;
+            default: e = launch_int8<bf16>(a, st); break;
         }
+        if (e != hipSuccess) return fail_msg(TAE_EHIP, hipGetErrorString(e));
         return (int)TAE_OK;
     });
 }
