@@ -30,6 +30,39 @@ __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cas
 template <class T, int V>
 __device__ __forceinline__ void store(T* p, const Pack<T, V>& a) { *reinterpret_cast<Pack<T, V>*>(p) = a; }
 
+// V adjacent elements as they were loaded, in whole registers: an element is taken out when it is used, so that a load stays in flight until
+// then and 16-bit elements need no registers of their own.
+template <class T, int V>
+struct Raw {
+    static constexpr int BYTES = sizeof(T) * V, WORDS = (BYTES + 3) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void from(const T* p) {
+        if constexpr (BYTES == 2) {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        } else if constexpr (BYTES == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (BYTES == 8) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            w[0] = u.x, w[1] = u.y;
+        } else {
+            static_assert(BYTES % 16 == 0, "whole 16-byte loads");
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return (float)__builtin_bit_cast(T, (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu));
+    }
+};
+
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }       // relative error 2^-22 |x| and up to one ulp
@@ -91,6 +124,27 @@ struct Width {
 constexpr int kGridX = 1 << 20;
 inline dim3 grid_of(int64_t n) { return n <= kGridX ? dim3((uint32_t)n) : dim3(kGridX, (uint32_t)ceil_div(n, kGridX)); }
 __device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
+
+// Quotients by a number that the host knows, with one product (Granlund and Montgomery 1994): for n < 2^31, n / d = (mulhi(n, m) + n) >> s
+// with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1.  Larger n are divided.
+struct Divisor {
+    uint32_t d, m, s;
+    Divisor() = default;
+    explicit Divisor(int64_t by) : d((uint32_t)by), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+    }
+    __device__ __forceinline__ void split(int64_t n, int64_t& quotient, int& rest) const {
+        if (n >> 31) {
+            quotient = n / d;
+            rest = (int)(n % d);
+        } else {
+            const uint32_t u = (uint32_t)n, q = (uint32_t)(((uint64_t)__umulhi(u, m) + u) >> s);
+            quotient = q;
+            rest = (int)(u - q * d);
+        }
+    }
+};
 
 // The launches of a C entry point: no exception leaves it, and a failed launch is an error of this call.
 template <class F>

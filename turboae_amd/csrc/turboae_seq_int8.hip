@@ -34,8 +34,9 @@ __device__ __forceinline__ Pack<int8_t, V> whole_numbers(const Pack<T, V>& p, fl
         o.v[i] = (int8_t)__float_as_int(r);
     }
     if (near) {
+        const float down = by > 1e36f ? 0x1p-10f : 1.0f;         // where 127 x would overflow
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = (int8_t)__float_as_int((float)p.v[i] * 127.0f / by + kMagic);
+        for (int i = 0; i < V; ++i) o.v[i] = (int8_t)__float_as_int((float)p.v[i] * down * 127.0f / (by * down) + kMagic);
     }
     return o;
 }

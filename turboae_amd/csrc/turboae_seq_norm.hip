@@ -14,7 +14,8 @@ struct NormArgs {
     const float *scale, *post_w, *post_b, *pre_w, *pre_b;
     void *out, *normed;
     int64_t rs_b, rs_r, bl_b, bl_r, ga_b, ga_r, ou_b, ou_r;
-    int rows, len, dim, center, gate_act;
+    int rows, dim, center, gate_act;
+    Divisor by_len;
     float eps, alpha;
 };
 
@@ -48,23 +49,28 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
     __shared__ float lds[16];
     const int lane = threadIdx.x % TPR;
     const int64_t row = block_index() * (THREADS / TPR) + threadIdx.x / TPR;
-    if (row >= a.rows) return;                  // whole workgroups, or with TPR = 64 whole waves, which meet no barrier
-    const int64_t b = row / a.len, t = row % a.len;
+    if (row >= a.rows) return;                  // whole workgroups, or with TPR <= 64 all lanes of a row, which meet no barrier
+    int64_t b;
+    int t;
+    a.by_len.split(row, b, t);
     const R* rs = (const R*)a.residual + b * a.rs_b + t * a.rs_r;
+    const T* bl = (const T*)a.block + b * a.bl_b + t * a.bl_r;
+    const T* ga = (const T*)a.gate + b * a.ga_b + t * a.ga_r;
     const float inv = 1.0f / (float)a.dim;
-    float r[NV][V];
+    // all of the row is on its way before any of it is used; lanes behind the row repeat its last elements
+    Raw<R, V> raw_r[NV];
+    Raw<T, V> raw_p[NV], raw_g[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int e = (j * TPR + lane) * V;
-        if (e < a.dim) {
-            const Pack<R, V> x = load<R, V>(rs + e);
+    for (int j = 0; j < NV; ++j) raw_r[j].from(rs + min((j * TPR + lane) * V, a.dim - V));
+    if (a.block) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) r[j][i] = (float)x.v[i];
-        } else {
+        for (int j = 0; j < NV; ++j) raw_p[j].from(bl + min((j * TPR + lane) * V, a.dim - V));
+        if (a.gate) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) r[j][i] = 0.0f;
+            for (int j = 0; j < NV; ++j) raw_g[j].from(ga + min((j * TPR + lane) * V, a.dim - V));
         }
     }
+    float r[NV][V];
     auto norm_of = [&](const float (&v)[NV][V], float& mean, float& rstd) {
         mean = 0.0f;
         float s = 0.0f;
@@ -85,24 +91,17 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
                 s = __builtin_fmaf(d, d, s);
             }
         }
-        rstd = 1.0f / sqrtf(row_sum<TPR, THREADS>(s, lds) * inv + a.eps);
+        rstd = __builtin_amdgcn_rsqf(row_sum<TPR, THREADS>(s, lds) * inv + a.eps);
+    };
+    auto unpack = [&](float (&v)[NV][V], auto& raw) {        // zeros behind the row
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j][i] = (j * TPR + lane) * V < a.dim ? raw[j][i] : 0.0f;
     };
     if (a.block) {
-        const T* bl = (const T*)a.block + b * a.bl_b + t * a.bl_r;
-        const T* ga = a.gate ? (const T*)a.gate + b * a.ga_b + t * a.ga_r : nullptr;
         float p[NV][V];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int e = (j * TPR + lane) * V;
-            if (e < a.dim) {
-                const Pack<T, V> x = load<T, V>(bl + e);
-#pragma unroll
-                for (int i = 0; i < V; ++i) p[j][i] = (float)x.v[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) p[j][i] = 0.0f;
-            }
-        }
+        unpack(p, raw_p);
         float mean = 0.0f, rstd = 1.0f;
         if (a.post_w) norm_of(p, mean, rstd);
 #pragma unroll
@@ -127,14 +126,20 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) f[i] *= w.v[i];
             }
-            if (ga) {
-                const Pack<T, V> g = load<T, V>(ga + e);
+            if (a.gate) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] *= gate_value((float)g.v[i], a.gate_act);
+                for (int i = 0; i < V; ++i) f[i] *= gate_value(raw_g[j][i], a.gate_act);
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) r[j][i] = __builtin_fmaf(a.alpha, f[i], r[j][i]);
+            for (int i = 0; i < V; ++i) p[j][i] = f[i];
         }
+        unpack(r, raw_r);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[j][i] = __builtin_fmaf(a.alpha, p[j][i], r[j][i]);
+    } else {
+        unpack(r, raw_r);
     }
     if (a.out) {
         R* o = (R*)a.out + b * a.ou_b + t * a.ou_r;
@@ -178,18 +183,21 @@ static void launch_norm_as(const NormArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((norm_residual_kernel<T, R, V, NV, TPR, THREADS>), grid_of(ceil_div(a.rows, THREADS / TPR)), dim3(THREADS), 0, st, a);
 }
 
-// Lanes and steps that hold a row: one wave for short rows, else as many lanes as leave each at most 32 elements.
+// Lanes and steps of V that hold a row: part of a wave for short rows, then a wave, then a workgroup.
 template <class T, class R, int V>
 static void launch_norm_width(const NormArgs& a, hipStream_t st) {
     const int vecs = (int)ceil_div(a.dim, V);
-    constexpr int M = 8 / V;                    // steps of V that are one step of 8
-    if (vecs <= 64 * M) launch_norm_as<T, R, V, M, 64, 256>(a, st);
+    constexpr int M = V == 1 ? 4 : 1;           // single elements: four for each lane at least
+    if (vecs <= 16 * M) launch_norm_as<T, R, V, M, 16, 256>(a, st);
+    else if (vecs <= 32 * M) launch_norm_as<T, R, V, M, 32, 256>(a, st);
+    else if (vecs <= 64 * M) launch_norm_as<T, R, V, M, 64, 256>(a, st);
     else if (vecs <= 128 * M) launch_norm_as<T, R, V, 2 * M, 64, 256>(a, st);
     else if (vecs <= 256 * M) launch_norm_as<T, R, V, M, 256, 256>(a, st);
     else if (vecs <= 512 * M) launch_norm_as<T, R, V, 2 * M, 256, 256>(a, st);
     else if (vecs <= 1024 * M) launch_norm_as<T, R, V, 4 * M, 256, 256>(a, st);
     else if (vecs <= 2048 * M) launch_norm_as<T, R, V, 2 * M, 1024, 1024>(a, st);
-    else launch_norm_as<T, R, V, 4 * M, 1024, 1024>(a, st);
+    else if (V == 8 || vecs <= 4096 * M) launch_norm_as<T, R, V, 4 * M, 1024, 1024>(a, st);
+    else if constexpr (V < 8) launch_norm_as<T, R, V, 8 * M, 1024, 1024>(a, st);
 }
 
 template <class T, class R>
@@ -234,7 +242,7 @@ extern "C" int tae_norm_residual(const tae_norm_args* p, void* stream) {
         if (width == 1 && p->dim % v == 0 && wt.fits(v * tb < 16 ? v * tb : 16) && wr.fits(v * rb < 16 ? v * rb : 16) && wf.fits(16)) width = v;
     NormArgs a{p->residual, p->block, p->gate, p->scale, p->post_weight, p->post_bias, p->pre_weight, p->pre_bias, p->residual_out, p->normed,
                p->residual_batch, p->residual_row, p->block_batch, p->block_row, p->gate_batch, p->gate_row, p->out_batch, p->out_row,
-               p->batch * p->len, p->len, p->dim, p->center ? 1 : 0, p->gate_act, p->eps, p->alpha};
+               p->batch * p->len, p->dim, p->center ? 1 : 0, p->gate_act, Divisor(p->len), p->eps, p->alpha};
     return guarded([&] {
         hipStream_t st = (hipStream_t)stream;
         const bool same = p->residual_dtype == p->dtype;

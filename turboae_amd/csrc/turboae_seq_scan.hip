@@ -12,7 +12,8 @@ struct ScanArgs {
     float* state_out;
     float *steps, *states;                       // workspace: (batch, pieces, channels) sums of d; (batch, pieces + 1, states, channels)
     int64_t x_b, x_r, dt_b, dt_r, b_b, b_r, c_b, c_r, z_b, z_r;
-    int len, channels, n, softplus, gate, groups, pieces, piece_len;      // groups of CW channels; pieces of piece_len positions
+    int len, channels, n, softplus, gate, pieces, piece_len;       // pieces of piece_len positions
+    Divisor by_groups, by_pieces;                                  // groups of channels; pieces
     int64_t blocks;
 };
 
@@ -79,12 +80,12 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
     constexpr int R = TT * CW / 4 / kScanThreads, RB = (TT * N + kScanThreads - 1) / kScanThreads;      // groups of four, elements for each thread
     static_assert(R >= 1 && TT * CW % (4 * kScanThreads) == 0, "a tile is whole groups of four for every thread");
     __shared__ float sd[2][CW * DS], sx[2][CW * DS], sb[2][N * DS], sc[ENDS ? 1 : 2][ENDS ? 4 : N * DS], sy[ENDS ? 1 : 2][ENDS ? 4 : CW * DS];
-    int64_t id = block_index();
+    const int64_t id = block_index();
     if (id >= q.blocks) return;
-    const int group = (int)(id % q.groups);
-    id /= q.groups;
-    const int piece = (int)(id % q.pieces);
-    const int64_t b = id / q.pieces;
+    int64_t rest, b;
+    int group, piece;
+    q.by_groups.split(id, rest, group);
+    q.by_pieces.split(rest, b, piece);
     const int tid = threadIdx.x, ch = tid / P, p = tid % P;
     const int e0 = group * CW, e = e0 + ch, E = q.channels;
     const bool mine = e < E;
@@ -329,12 +330,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_lane_kernel(ScanArgs q) {
     __shared__ alignas(16) float lds[kScanThreads / 64][2][kAhead * W];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float(*rows)[kAhead * W] = lds[wave];
-    int64_t id = block_index() * (kScanThreads / 64) + wave;
+    const int64_t id = block_index() * (kScanThreads / 64) + wave;
     if (id >= q.blocks) return;
-    const int group = (int)(id % q.groups);
-    id /= q.groups;
-    const int piece = (int)(id % q.pieces);
-    const int64_t b = id / q.pieces;
+    int64_t rest, b;
+    int group, piece;
+    q.by_groups.split(id, rest, group);
+    q.by_pieces.split(rest, b, piece);
     const int lane = threadIdx.x & 63, p = lane % P, n0 = p * N, E = q.channels, e = group * CW + lane / P, ec = min(e, E - 1);
     const bool mine = e < E;
     const int n = q.lengths ? min(max(q.lengths[b], 0), q.len) : q.len;
@@ -537,66 +538,88 @@ __global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs q, int
 }
 
 // One position: bound by reading and writing the states.  P lanes share a channel, each holds V adjacent states; they keep A in registers
-// and walk `each` sequences.
-template <class T, int P, int V>
-__global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int batch, int each) {
+// for EACH sequences, whose operands are all on their way before the first is worked on.
+template <class T, int P, int V, int EACH>
+__global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int batch) {
     constexpr int CW = kScanThreads / P;
     const int64_t id = block_index();
     if (id >= q.blocks) return;
-    const int tid = threadIdx.x, p = tid % P, e = (int)(id % q.groups) * CW + tid / P, E = q.channels;
-    const int b0 = (int)(id / q.groups) * each, b1 = min(b0 + each, batch);
+    int64_t row;
+    int group;
+    q.by_groups.split(id, row, group);
+    const int tid = threadIdx.x, p = tid % P, e = group * CW + tid / P, E = q.channels, b0 = (int)row * EACH;
     const int k = p * V;                         // V = 4: states are whole groups of four
-    const int ec = min(e, E - 1);                // lanes without a channel stay for the sums over lanes
+    const int ec = min(e, E - 1), kc = min(k, q.n - V);      // lanes without a channel or a state stay for the sums over lanes
     const bool mine = e < E && k < q.n;
-    Pack<float, V> a2{};
-    if (mine) a2 = load<float, V>(q.a + (int64_t)e * q.n + k);
+    const Pack<float, V> a = load<float, V>(q.a + (int64_t)ec * q.n + kc);
     const float bias = q.dt_bias ? q.dt_bias[ec] : 0.0f, dcoef = q.d ? q.d[ec] : 0.0f;
-    for (int b = b0; b < b1; ++b) {
-        const int64_t at = ((int64_t)b * E + e) * q.n + k;
-        Pack<float, V> h{};
-        if (mine && q.state) h = load<float, V>(q.state + at);
-        float out = 0.0f;
-        if (!q.lengths || q.lengths[b] > 0) {
-            const float x = (float)((const T*)q.x)[b * q.x_b + ec];
-            float d = (float)((const T*)q.dt)[b * q.dt_b + ec] + bias;
-            if (q.softplus) d = softplus(d);
-            if (mine) {
-                const Pack<T, V> bm = load<T, V>((const T*)q.b + b * q.b_b + k), cm = load<T, V>((const T*)q.c + b * q.c_b + k);
+    Pack<float, V> h[EACH];
+    Raw<T, 1> x[EACH], dt[EACH], z[EACH];
+    Raw<T, V> bm[EACH], cm[EACH];
+    bool on[EACH];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    h.v[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * (a2.v[i] * kLog2e)), h.v[i], d * x * (float)bm.v[i]);
-                    out = __builtin_fmaf(h.v[i], (float)cm.v[i], out);
-                }
+    for (int i = 0; i < EACH; ++i) {
+        const int64_t b = min(b0 + i, batch - 1);
+        on[i] = !q.lengths || q.lengths[b] > 0;
+        if (q.state) h[i] = load<float, V>(q.state + (b * E + ec) * q.n + kc);
+        else h[i] = Pack<float, V>{};
+        if (on[i]) {                             // what is padding is not read
+            x[i].from((const T*)q.x + b * q.x_b + ec);
+            dt[i].from((const T*)q.dt + b * q.dt_b + ec);
+            z[i].from((const T*)q.z + b * q.z_b + ec);
+            bm[i].from((const T*)q.b + b * q.b_b + kc);
+            cm[i].from((const T*)q.c + b * q.c_b + kc);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int64_t b = b0 + i;
+        float out = 0.0f;
+        if (on[i]) {
+            float d = dt[i][0] + bias;
+            if (q.softplus) d = softplus(d);
+            const float dx = d * x[i][0];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h[i].v[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * (a.v[j] * kLog2e)), h[i].v[j], dx * bm[i][j]);
+                if (mine) out = __builtin_fmaf(h[i].v[j], cm[i][j], out);
             }
             out = lanes_sum<P>(out);
-            out = __builtin_fmaf(dcoef, x, out);
-            if (q.gate) out *= silu((float)((const T*)q.z)[b * q.z_b + ec]);
+            out = __builtin_fmaf(dcoef, x[i][0], out);
+            if (q.gate) out *= silu(z[i][0]);
         }
-        if (p == 0 && e < E) ((T*)q.y)[(int64_t)b * E + e] = (T)out;
-        if (mine) store<float, V>(q.state_out + at, h);
+        if (b < batch && e < E) {
+            if (p == 0) ((T*)q.y)[b * E + e] = (T)out;
+            if (mine) store<float, V>(q.state_out + (b * E + e) * q.n + k, h[i]);
+        }
     }
 }
 
-template <class T, int V>
+template <class T, int V, int EACH>
 static int launch_step(ScanArgs a, int batch, hipStream_t st) {
     int lanes = 1;
     while (lanes * V < a.n) lanes *= 2;
-    a.groups = (int)ceil_div(a.channels, kScanThreads / lanes);
-    // up to four sequences for each workgroup, so that A is read once for them, as long as 1024 workgroups remain
-    const int each = (int)std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)a.groups * batch / 1024));
-    a.blocks = a.groups * ceil_div(batch, each);
+    const int64_t groups = ceil_div(a.channels, kScanThreads / lanes);
+    a.by_groups = Divisor(groups);
+    a.blocks = groups * ceil_div(batch, EACH);
     if (a.blocks > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "selective_scan: the batch is too large for one call");
     const dim3 grid = grid_of(a.blocks), block(kScanThreads);
     switch (lanes) {
-        case 1: hipLaunchKernelGGL((scan_step_kernel<T, 1, V>), grid, block, 0, st, a, batch, each); break;
-        case 2: hipLaunchKernelGGL((scan_step_kernel<T, 2, V>), grid, block, 0, st, a, batch, each); break;
-        case 4: hipLaunchKernelGGL((scan_step_kernel<T, 4, V>), grid, block, 0, st, a, batch, each); break;
-        case 8: hipLaunchKernelGGL((scan_step_kernel<T, 8, V>), grid, block, 0, st, a, batch, each); break;
-        case 16: hipLaunchKernelGGL((scan_step_kernel<T, 16, V>), grid, block, 0, st, a, batch, each); break;
-        case 32: hipLaunchKernelGGL((scan_step_kernel<T, 32, V>), grid, block, 0, st, a, batch, each); break;
-        default: hipLaunchKernelGGL((scan_step_kernel<T, 64, V>), grid, block, 0, st, a, batch, each); break;
+        case 1: hipLaunchKernelGGL((scan_step_kernel<T, 1, V, EACH>), grid, block, 0, st, a, batch); break;
+        case 2: hipLaunchKernelGGL((scan_step_kernel<T, 2, V, EACH>), grid, block, 0, st, a, batch); break;
+        case 4: hipLaunchKernelGGL((scan_step_kernel<T, 4, V, EACH>), grid, block, 0, st, a, batch); break;
+        case 8: hipLaunchKernelGGL((scan_step_kernel<T, 8, V, EACH>), grid, block, 0, st, a, batch); break;
+        case 16: hipLaunchKernelGGL((scan_step_kernel<T, 16, V, EACH>), grid, block, 0, st, a, batch); break;
+        case 32: hipLaunchKernelGGL((scan_step_kernel<T, 32, V, EACH>), grid, block, 0, st, a, batch); break;
+        default: hipLaunchKernelGGL((scan_step_kernel<T, 64, V, EACH>), grid, block, 0, st, a, batch); break;
     }
     return TAE_OK;
+}
+
+// Four sequences for each workgroup, so that A is read once for them, as long as two workgroups for each CU remain.
+template <class T, int V>
+static int launch_steps(const ScanArgs& a, int batch, hipStream_t st) {
+    return batch >= 4 && (int64_t)a.channels * a.n / V * batch >= 4 * 512 * kScanThreads ? launch_step<T, V, 4>(a, batch, st) : launch_step<T, V, 1>(a, batch, st);
 }
 
 // How a call is cut: P lanes for a channel, each with S states, by scan_lane_kernel or (tiled) selective_scan_kernel, and pieces.
@@ -685,7 +708,7 @@ static int launch_lane(const ScanArgs& a, int64_t batch, hipStream_t st) {
 
 template <class T>
 static int launch_scan_plan(const ScanArgs& a, const ScanPlan& s, bool v, int batch, hipStream_t st) {
-    if (a.len == 1) return v ? launch_step<T, 4>(a, batch, st) : launch_step<T, 1>(a, batch, st);
+    if (a.len == 1) return v ? launch_steps<T, 4>(a, batch, st) : launch_steps<T, 1>(a, batch, st);
     switch (s.tiled * 10000 + s.lanes * 100 + s.per_lane) {
         case 104: return launch_lane<T, 4, 1>(a, batch, st);
         case 108: return launch_lane<T, 8, 1>(a, batch, st);
@@ -742,7 +765,7 @@ int tae_selective_scan(const tae_scan_args* p, void* stream) {
     ScanArgs a{p->x, p->dt, p->b, p->c, p->z ? p->z : p->x, p->a, p->d, p->dt_bias, p->state, p->lengths, p->y, p->state_out,
                s.bytes ? (float*)p->workspace : nullptr, s.bytes ? (float*)((char*)p->workspace + s.steps_bytes) : nullptr,
                p->x_batch, p->x_row, p->dt_batch, p->dt_row, p->b_batch, p->b_row, p->c_batch, p->c_row, p->z ? p->z_batch : p->x_batch, p->z ? p->z_row : p->x_row,
-               p->len, p->channels, p->states, p->softplus ? 1 : 0, p->z ? 1 : 0, s.groups, s.pieces, s.piece_len, (int64_t)p->batch * s.groups * s.pieces};
+               p->len, p->channels, p->states, p->softplus ? 1 : 0, p->z ? 1 : 0, s.pieces, s.piece_len, Divisor(s.groups), Divisor(s.pieces), (int64_t)p->batch * s.groups * s.pieces};
     const size_t four = 4 * dtype_bytes(p->dtype);
     Width w(dtype_bytes(p->dtype));
     w.elements(p->channels).pointer(p->x).pointer(p->dt).pointer(p->z).pointer(p->y).elements(p->x_batch).elements(p->x_row).elements(p->dt_batch).elements(p->dt_row);

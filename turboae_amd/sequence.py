@@ -32,11 +32,16 @@ _ACT = {"linear": 1, "tanh": 2, "sigmoid": 5, "silu": 6}                        
 __all__ = ["causal_conv", "selective_scan", "norm_residual", "quantize_int8", "int8_linear", "token_logprobs"]
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _Call:
-    """The checks that every tensor of a call goes through, against the first of them."""
+    """The checks that every tensor of a call goes through, against the first of them; a call of a single token costs little more."""
+
+    __slots__ = ("name", "device", "dtype", "grad")
 
     def __init__(self, name: str, first: torch.Tensor):
-        if not isinstance(first, torch.Tensor) or first.device.type != "cuda":
+        if not isinstance(first, torch.Tensor) or not first.is_cuda:
             raise _lib.TurboAEError(f"{name}: needs tensors on a ROCm GPU device (no CPU fallback)")
         if first.dtype not in _DTYPE:
             raise ValueError(f"{name}: float32, float16 or bfloat16 wanted, got {first.dtype}")
@@ -46,13 +51,13 @@ class _Call:
         """Address of a tensor after its checks (None for None): shape, type, device, adjacent last elements; dense: contiguous."""
         if t is None:
             return None
-        if tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device:
-            raise ValueError(f"{self.name}: {what} must be {dtype} of shape {shape} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if dense:
-            if not t.is_contiguous():
+        if t.shape != shape or t.dtype is not dtype or t.device != self.device:
+            raise ValueError(f"{self.name}: {what} must be {dtype} of shape {tuple(shape)} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if not t.is_contiguous():
+            if dense:
                 raise ValueError(f"{self.name}: {what} must be contiguous")
-        elif shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{self.name}: adjacent elements of {what}'s last dimension must be adjacent in memory")
+            if shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"{self.name}: adjacent elements of {what}'s last dimension must be adjacent in memory")
         if self.grad and t.requires_grad:
             raise ValueError(f"{self.name}: {what} requires a gradient, but this path is inference only (call it under torch.no_grad())")
         return t.data_ptr()
@@ -74,25 +79,25 @@ class _Call:
         return w
 
     def run(self, entry, *args) -> None:
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        if torch.cuda.current_device() == self.device.index:
-            rc = entry(*args, stream)
+        index = self.device.index
+        if torch.cuda.current_device() == index:
+            rc = entry(*args, _raw_stream(index))
         else:
-            with torch.cuda.device(self.device):
-                rc = entry(*args, stream)
+            with torch.cuda.device(index):
+                rc = entry(*args, _raw_stream(index))
         if rc:
             _lib.check(rc)
 
 
 def _sequence(name: str, what: str, t: torch.Tensor) -> Tuple[int, int, int]:
-    if t.dim() != 3 or 0 in t.shape:
+    if t.dim() != 3 or t.numel() == 0:
         raise ValueError(f"{name}: {what} must have shape (batch, len, channels), none of them 0, got {tuple(t.shape)}")
-    return t.shape[0], t.shape[1], t.shape[2]
+    return t.shape
 
 
 def _strides(t: Optional[torch.Tensor]) -> Tuple[int, int]:
     """Distances between sequences and between positions; a tensor of another shape is refused by its own check."""
-    return (t.stride(0), t.stride(1)) if t is not None and t.dim() == 3 else (0, 0)
+    return t.stride()[:2] if t is not None and t.dim() == 3 else (0, 0)
 
 
 def _in_place_or_apart(name: str, source: Optional[torch.Tensor], out: torch.Tensor) -> None:
