@@ -169,16 +169,16 @@ __device__ __forceinline__ void wait_copies() {             // all but the last 
 // BM x BN outputs at a time for each workgroup of WM x WN waves, 64 weight rows for each wave.
 //
 // Bound by the matrix instructions.  A workgroup takes tile after tile without a break: the slabs of 128 inputs of all its tiles are one
-// stream through two LDS buffers, copied directly, whole 128-byte lines at a time.  The one barrier of a slab stands behind its last
-// fragment reads, a quarter of its products before its end: there the next slab has arrived, this slab's buffer is free for the one after
-// it, and the next slab's first fragments are read during the rest of the products.  A tile's results are stored while the next tile is
+// stream through STAGES LDS buffers, copied directly, whole 128-byte lines at a time.  The one barrier of a slab stands behind its last
+// fragment reads, a quarter of its products before its end: there the next slab has arrived, this slab's buffer is free for the one
+// STAGES further, and the next slab's first fragments are read during the rest of the products.  A tile's results are stored while the next tile is
 // under way.  A row's eight 16-byte pieces are permuted by its number (by which piece a lane copies), so that the 16 lanes which read LDS
 // together touch all banks.  Weight rows are dealt to fragments such that a lane ends up with 16 adjacent outputs.  Workgroups of one XCD
 // (every eighth) take adjacent tiles, eight rows of tiles high, and share operands in its L2.
-template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64, 2) void int8_linear_kernel(Int8Args a) {
-    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = 4, ROWS = BM + BN, PIECES = ROWS / 8 / WAVES, STAGE = ROWS * 128;
-    static_assert(BN / WN == 64 && ROWS % (8 * WAVES) == 0 && BM % (8 * PIECES) == 0, "whole pieces of one operand for each wave");
+template <class T, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64, BM / WM * (BN / WN) > 8192 ? 1 : 2) void int8_linear_kernel(Int8Args a) {
+    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, ROWS = BM + BN, PIECES = ROWS / 8 / WAVES, STAGE = ROWS * 128;
+    static_assert(BN / WN % 64 == 0 && ROWS % (8 * WAVES) == 0 && BM % (8 * PIECES) == 0, "whole pieces of one operand for each wave");
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     // this workgroup's tiles: of its XCD's share, every (workgroups of the XCD)-th
@@ -228,35 +228,38 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_linear_kernel(Int8Args a
     // pieces q and 4 + q of row r16 for the two halves of a slab
     const int r16 = lane & 15, half[2] = {r16 * 128 + (((lane >> 4) ^ r16) & 7) * 16, r16 * 128 + (((lane >> 4 | 4) ^ r16) & 7) * 16};
     i32x4 wf[NF], wf_next[NF], qf[MF], qf_next[2], acc[NF][MF] = {};
-    auto weight = [&](const char* p, int f) { return *(const i32x4*)(p + (BM + wn * 64 + f * 16) * 128); };
+    auto weight = [&](const char* p, int f) { return *(const i32x4*)(p + (BM + (wn * NF + f) * 16) * 128); };
     auto x = [&](const char* p, int f) { return *(const i32x4*)(p + (wm * MF + f) * 2048); };
     int tile = 0, slab = 0, stage = 0, m0, n0;
     auto results = [&]() {
-        const int n = n0 + wn * 64 + (lane >> 4) * 16;
-        const Outputs<T, 16> outputs(a, n);
         float sm[MF];
 #pragma unroll
         for (int i = 0; i < MF; ++i) sm[i] = a.scale[min(m0 + (wm * MF + i) * 16 + r16, a.m - 1)];
         const bool whole = a.wide && n0 + BN <= a.n;
 #pragma unroll
-        for (int i = 0; i < MF; ++i) {
-            const int m = m0 + (wm * MF + i) * 16 + r16;
-            int sum[16];
+        for (int block = 0; block < NF / 4; ++block) {
+            const int n = n0 + (wn * NF / 4 + block) * 64 + (lane >> 4) * 16;
+            const Outputs<T, 16> outputs(a, n);
 #pragma unroll
-            for (int f = 0; f < NF; ++f)
+            for (int i = 0; i < MF; ++i) {
+                const int m = m0 + (wm * MF + i) * 16 + r16;
+                int sum[16];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    sum[f * 4 + r] = acc[f][i][r];
-                    acc[f][i][r] = 0;
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        sum[f * 4 + r] = acc[block * 4 + f][i][r];
+                        acc[block * 4 + f][i][r] = 0;
+                    }
+                const Pack<T, 16> out = outputs.row(sum, sm[i]);
+                T* y = (T*)a.y + (int64_t)m * a.n + n;
+                if (whole) {
+                    if (m < a.m) store_once(y, out);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        if (m < a.m && n + c < a.n) y[c] = out.v[c];
                 }
-            const Pack<T, 16> out = outputs.row(sum, sm[i]);
-            T* y = (T*)a.y + (int64_t)m * a.n + n;
-            if (whole) {
-                if (m < a.m) store_once(y, out);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    if (m < a.m && n + c < a.n) y[c] = out.v[c];
             }
         }
     };
@@ -281,9 +284,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_linear_kernel(Int8Args a
     };
     place(0, m0, n0);
     open(0);
-    copy(0);
-    copy(1);
-    wait_copies<PIECES>();
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) copy(s);
+    wait_copies<(STAGES - 1) * PIECES>();
     first(lds + half[0]);
     advance();
     for (;;) {
@@ -310,9 +313,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_linear_kernel(Int8Args a
             __builtin_amdgcn_sched_group_barrier(0x008, EARLY * NF / (MF - 2), 1);
         }
         // all fragments of this slab have been read, by every wave, and all copies of the next one have arrived
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_copies<(STAGES - 2) * PIECES>();
         copy(stage);
-        stage ^= 1;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
         first(lds + stage * STAGE + half[0]);
         multiply(EARLY, MF);
         advance();
@@ -325,91 +329,110 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_linear_kernel(Int8Args a
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no copy is under way when the workgroup's LDS is given away
 }
 
-// Few rows of x: bound by reading the weights.  16 weight rows and up to 16 MF rows of x for each workgroup; its eight waves share the inputs
-// and join their sums, exact in any order, in LDS.  Both operands come straight from memory (x from L2), kDeep slabs in flight.
-template <class T, int MF>
+// Few rows of x: bound by reading the weights.  16 NF weight rows and up to 16 MF rows of x for each workgroup; its eight waves share the
+// inputs and join their sums, exact in any order, in LDS.  Both operands come straight from memory (x from L2), DEEP slabs of 64 in flight.
+template <class T, int MF, int NF, int DEEP>
 __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
-    constexpr int kDeep = MF == 1 ? 8 : 4;
-    __shared__ i32x4 part[8][MF][64];
+    constexpr int FRAGMENTS = MF * NF, ROUND = FRAGMENTS < 8 ? FRAGMENTS : 8;          // joined at once
+    __shared__ i32x4 part[8][ROUND][64];
     const int64_t id = block_index();
     if (id >= a.blocks) return;
-    const int n0 = (int)(id % a.tiles_n) * 16, m0 = (int)(id / a.tiles_n) * 16 * MF;
+    const int n0 = (int)(id % a.tiles_n) * 16 * NF, m0 = (int)(id / a.tiles_n) * 16 * MF;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kk = (lane >> 4) * 16;
     const int slabs = (a.k + 63) / 64, each = (slabs + 7) / 8, begin = wave * each, end = min(begin + each, slabs);
-    const int8_t* w = a.w + (int64_t)min(n0 + r16, a.n - 1) * a.w_r;
-    const int8_t* q[MF];
+    const int8_t *w[NF], *q[MF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) w[f] = a.w + (int64_t)min(n0 + f * 16 + r16, a.n - 1) * a.w_r;
 #pragma unroll
     for (int i = 0; i < MF; ++i) q[i] = a.q + (int64_t)min(m0 + i * 16 + r16, a.m - 1) * a.q_r;
-    i32x4 acc[MF] = {};
+    i32x4 acc[NF][MF] = {};
     const int last = (a.k - 1) & ~15;            // the last 16 bytes of a row that may be read; q is zero where they repeat
-    for (int s0 = begin; s0 < end; s0 += kDeep) {
-        i32x4 wv[kDeep], qv[kDeep][MF];
+    for (int s0 = begin; s0 < end; s0 += DEEP) {
+        i32x4 wv[DEEP][NF], qv[DEEP][MF];
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
+        for (int d = 0; d < DEEP; ++d) {
             const int k = min(s0 + d, end - 1) * 64 + kk;
-            wv[d] = *(const i32x4*)(w + min(k, last));
+#pragma unroll
+            for (int f = 0; f < NF; ++f) wv[d][f] = *(const i32x4*)(w[f] + min(k, last));
 #pragma unroll
             for (int i = 0; i < MF; ++i) qv[d][i] = *(const i32x4*)(q[i] + k);
         }
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
+        for (int d = 0; d < DEEP; ++d) {
             if (s0 + d < end) {
 #pragma unroll
-                for (int i = 0; i < MF; ++i) acc[i] = mfma64(wv[d], qv[d][i], acc[i]);
+                for (int i = 0; i < MF; ++i)
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) acc[f][i] = mfma64(wv[d][f], qv[d][i], acc[f][i]);
             }
         }
     }
+    // fragment f, i is number f + NF i; a wave finishes those whose number is its own modulo 8
 #pragma unroll
-    for (int i = 0; i < MF; ++i) part[wave][i][lane] = acc[i];
-    __syncthreads();
-    if (wave >= MF) return;
-    i32x4 sum = part[0][wave][lane];
+    for (int first = 0; first < FRAGMENTS; first += ROUND) {
+        if (first > 0) __syncthreads();          // the last round has been read
 #pragma unroll
-    for (int u = 1; u < 8; ++u) sum += part[u][wave][lane];
-    const int m = m0 + wave * 16 + r16, n = n0 + (lane >> 4) * 4;
-    if (m >= a.m || n >= a.n) return;
-    const Pack<T, 4> out = Outputs<T, 4>(a, n).row({sum[0], sum[1], sum[2], sum[3]}, a.scale[m]);
-    T* y = (T*)a.y + (int64_t)m * a.n + n;
-    if (a.wide) {                                // outputs come in whole groups of four
-        store<T, 4>(y, out);
-    } else {
+        for (int j = 0; j < ROUND; ++j) part[wave][j][lane] = acc[(first + j) % NF][(first + j) / NF];
+        __syncthreads();
+        if (wave >= ROUND) continue;
+        i32x4 sum = part[0][wave][lane];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (n + c < a.n) y[c] = out.v[c];
+        for (int u = 1; u < 8; ++u) sum += part[u][wave][lane];
+        const int m = m0 + (first + wave) / NF * 16 + r16, n = n0 + (first + wave) % NF * 16 + (lane >> 4) * 4;
+        if (m >= a.m || n >= a.n) continue;
+        const Pack<T, 4> out = Outputs<T, 4>(a, n).row({sum[0], sum[1], sum[2], sum[3]}, a.scale[m]);
+        T* y = (T*)a.y + (int64_t)m * a.n + n;
+        if (a.wide) {                            // outputs come in whole groups of four
+            store<T, 4>(y, out);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (n + c < a.n) y[c] = out.v[c];
+        }
     }
 }
 
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, int BM, int BN, int WM, int WN, int STAGES>
 static hipError_t launch_tiles(Int8Args a, hipStream_t st) {
-    constexpr int bytes = 2 * (BM + BN) * 128;
+    constexpr int bytes = STAGES * (BM + BN) * 128;
     a.tiles_m = ceil_div(a.m, BM);
     a.tiles_n = (int)ceil_div(a.n, BN);
     a.blocks = a.tiles_m * a.tiles_n;
-    const void* kernel = reinterpret_cast<const void*>(int8_linear_kernel<T, BM, BN, WM, WN>);
+    const void* kernel = reinterpret_cast<const void*>(int8_linear_kernel<T, BM, BN, WM, WN, STAGES>);
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);        // of the current device
     if (e != hipSuccess) return e;
     const int64_t resident = 256 * (160 * 1024 / bytes);     // workgroups that 256 CUs hold at once
-    hipLaunchKernelGGL((int8_linear_kernel<T, BM, BN, WM, WN>), dim3((uint32_t)std::min(a.blocks, resident)), dim3(WM * WN * 64), bytes, st, a);
+    hipLaunchKernelGGL((int8_linear_kernel<T, BM, BN, WM, WN, STAGES>), dim3((uint32_t)std::min(a.blocks, resident)), dim3(WM * WN * 64), bytes, st, a);
     return hipSuccess;
 }
 
-template <class T, int MF>
+template <class T, int MF, int NF, int DEEP>
 static hipError_t launch_few(Int8Args a, hipStream_t st) {
     a.tiles_m = ceil_div(a.m, 16 * MF);
-    a.tiles_n = (int)ceil_div(a.n, 16);
+    a.tiles_n = (int)ceil_div(a.n, 16 * NF);
     a.blocks = a.tiles_m * a.tiles_n;
-    hipLaunchKernelGGL((int8_few_kernel<T, MF>), grid_of(a.blocks), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((int8_few_kernel<T, MF, NF, DEEP>), grid_of(a.blocks), dim3(512), 0, st, a);
     return hipSuccess;
 }
 
+// Which form: measured whole calls in bf16, in us -
+//     4096 inputs and outputs, rows       64  128  256  512  1024  2048  3000  4096
+//     few, 32 x 32 a workgroup            15   22   37   67   126   243
+//     few, 64 x 32                        18   19   30   54   100   190
+//     tiles of 128 x 128, four buffers    23   23   24   27    30    51    72    98
+//     the same, two buffers, two for a CU 25   26   27   30    34    47    67    91
+//     tiles of 256 x 256                                             57    63    83
+//     8000 rows, 4000 outputs, inputs    200  500  1000  2000
+//     128 x 128, four / two buffers    41/35  53/47  70/63  107/96         256 x 256   57  65  78  101
+// and with 256 rows, 16000 inputs and 512 outputs, where tiles are too few for the CUs, few 43, tiles of 128 x 128 71.
 template <class T>
 static hipError_t launch_int8(const Int8Args& a, hipStream_t st) {
-    if (a.m <= 16) return launch_few<T, 1>(a, st);
-    if (a.m <= 32) return launch_few<T, 2>(a, st);
+    if (a.m <= 16) return launch_few<T, 1, 1, 8>(a, st);
     const int64_t large = ceil_div(a.m, 256) * ceil_div(a.n, 256), small = ceil_div(a.m, 128) * ceil_div(a.n, 128);
-    if (large >= 192) return launch_tiles<T, 256, 256, 2, 4>(a, st);
-    if (a.m <= 128 || small < 128) return launch_few<T, 4>(a, st);
-    return launch_tiles<T, 128, 128, 2, 2>(a, st);
+    if (a.m <= 64 || (small < 64 && a.k >= 4096)) return launch_few<T, 2, 2, 4>(a, st);
+    if (a.m <= 128) return launch_few<T, 4, 2, 4>(a, st);
+    if (large >= 192 && a.k >= 4096) return launch_tiles<T, 256, 256, 2, 4, 2>(a, st);
+    return small <= 256 ? launch_tiles<T, 128, 128, 2, 2, 4>(a, st) : launch_tiles<T, 128, 128, 2, 2, 2>(a, st);
 }
 
 // Rows 1024 bytes and multiples apart would send a slab's lines of all rows to few channels of L2.
