@@ -328,7 +328,8 @@ TAE_API int tae_debug_split_f16(const float* x, size_t n, float scale, uint16_t*
  *  - activations are TAE_DTYPE_*, the parameters named `float` below fp32; sums, norms, softmax statistics and states are fp32 or wider, and
  *    every result is rounded once, when it is stored;
  *  - tensors of activations are (batch, len, channels) with adjacent channels; `*_batch` / `*_row` are the distances, in elements, between
- *    sequences and between positions, so a slice of a wider tensor needs no copy.  Outputs are contiguous, except norm_residual's residual;
+ *    sequences and between positions, so a slice of a wider tensor needs no copy.  Outputs are contiguous, except norm_residual's residual,
+ *    and overlap neither inputs nor each other, except where that is named; pointers are aligned to their elements;
  *  - `lengths` (device, int32 per sequence; NULL: all of `len`) marks padding: positions at or behind lengths[b] (clamped to 0..len) are not
  *    read, their outputs are zero, and a final state is the one after the last position in front of them;
  *  - workspaces belong to the caller (16-byte aligned, tae_*_workspace bytes) and must not be shared by calls that can run at the same time;
@@ -391,7 +392,9 @@ TAE_API int tae_selective_scan(const tae_scan_args* args, void* stream);
  *     p = post ? norm(block) * post_weight + post_bias : block
  *     r = residual + alpha * scale * gate_act(gate) * p          (block NULL: r = residual)
  *     normed = norm(r) * pre_weight + pre_bias                   (of r before its rounding)
- * norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps), mean = 0 with center = 0.  residual_out may be residual itself (same strides). */
+ * norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps), mean = 0 with center = 0.  residual_out may be residual itself (same strides).
+ * Squares are summed in fp32: norm is 0 for a row whose
+ * sum of squares is not finite there. */
 typedef struct tae_norm_args {
     int32_t struct_size;          /* = sizeof(tae_norm_args) */
     int32_t dtype;                /* block, gate, normed */
@@ -399,7 +402,7 @@ typedef struct tae_norm_args {
     int32_t batch, len, dim;      /* dim 1..32768 */
     int32_t center;               /* 1: subtract the mean */
     int32_t gate_act;             /* TAE_ACT_LINEAR, TANH, SIGMOID or SILU */
-    float eps;                    /* > 0 */
+    float eps;                    /* > 0, not subnormal */
     float alpha;
     int64_t residual_batch, residual_row, block_batch, block_row;
     int64_t gate_batch, gate_row; /* gate_row = 0: one gate for each sequence */

@@ -75,6 +75,11 @@ def logprobs():
     (logprobs, "tae_token_logprobs", "2^21", dict(vocab=(1 << 21) + 1)), (logprobs, "tae_token_logprobs", "top", dict(top=33)), (logprobs, "tae_token_logprobs", "token_bytes", dict(token_bytes=2)),
     (logprobs, "tae_token_logprobs", "NULL", dict(tokens=None)), (logprobs, "tae_token_logprobs", "top needs", dict(top_ids=None)),
     (logprobs, "tae_token_logprobs", "aligned", dict(logits=PTR + 2)), (logprobs, "tae_token_logprobs", "workspace", dict()),
+    (conv, "tae_causal_conv", "aligned", dict(dtype=1, x=PTR + 1)), (conv, "tae_causal_conv", "aligned", dict(weight=PTR + 2)), (conv, "tae_causal_conv", "aligned", dict(state_out=PTR + 2)),
+    (scan, "tae_selective_scan", "aligned", dict(dtype=2, z=PTR + 1)), (scan, "tae_selective_scan", "aligned", dict(state_out=PTR + 2)), (scan, "tae_selective_scan", "aligned", dict(lengths=PTR + 1)),
+    (norm, "tae_norm_residual", "aligned", dict(block=PTR + 2)), (norm, "tae_norm_residual", "aligned", dict(scale=PTR + 1)), (norm, "tae_norm_residual", "subnormal", dict(eps=1e-40)),
+    (int8, "tae_int8_linear", "aligned", dict(x=PTR + 2, workspace=PTR, workspace_bytes=1 << 20)), (int8, "tae_int8_linear", "aligned", dict(bias=PTR + 2, workspace=PTR, workspace_bytes=1 << 20)),
+    (logprobs, "tae_token_logprobs", "aligned", dict(top_ids=PTR + 4)), (logprobs, "tae_token_logprobs", "too many rows", dict(rows=(1 << 31) - 1, vocab=1 << 21, workspace=PTR, workspace_bytes=1 << 62)),
 ])
 def test_bad_arguments_are_refused(make, entry, match, change):
     refused(getattr(_lib.load(), entry), make(), match, **change)

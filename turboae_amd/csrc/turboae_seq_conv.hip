@@ -139,6 +139,8 @@ extern "C" int tae_causal_conv(const tae_conv_args* p, void* stream) {
     if (p->act != TAE_ACT_LINEAR && p->act != TAE_ACT_SILU) return fail_msg(TAE_EINVAL, "causal_conv: act must be linear or silu");
     if (!p->x || !p->weight || !p->y) return fail_msg(TAE_EINVAL, "causal_conv: x, weight and y must not be NULL");
     const size_t tb = dtype_bytes(p->dtype);
+    if (!elements_aligned(tb, p->x, p->state, p->y, p->state_out) || !elements_aligned(4, p->weight, p->bias, p->lengths))
+        return fail_msg(TAE_EINVAL, "causal_conv: a pointer is not aligned to its elements");
     Width w(tb);
     w.elements(p->channels).elements(p->x_batch).elements(p->x_row).pointer(p->x).pointer(p->y).pointer(p->state).pointer(p->state_out);
     const int vec = w.fits(16) ? (int)(16 / tb) : w.fits(4) ? (int)(4 / tb) : 1;

@@ -457,6 +457,7 @@ int tae_quantize_int8(int32_t dtype, const void* x, int64_t x_row, int32_t rows,
     if (!x || !q || !scale) return fail_msg(TAE_EINVAL, "quantize_int8: x, q and scale must not be NULL");
     if (rows < 1 || cols < 1 || cols > (1 << 30)) return fail_msg(TAE_EINVAL, "quantize_int8: rows must be >= 1, cols in 1..2^30");
     if (q_row < cols || q_row % 16 || q_row > (1 << 30) + 1024 || !aligned(q, 16)) return fail_msg(TAE_EINVAL, "quantize_int8: q rows start on 16-byte boundaries and hold cols values");
+    if (!elements_aligned(dtype_bytes(dtype), x) || !elements_aligned(4, scale)) return fail_msg(TAE_EINVAL, "quantize_int8: a pointer is not aligned to its elements");
     return guarded([&] {
         launch_quantize_dtype(QuantArgs{x, q, scale, x_row, q_row, rows, cols}, dtype, (hipStream_t)stream);
         return (int)TAE_OK;
@@ -479,6 +480,7 @@ int tae_int8_linear(const tae_int8_args* p, void* stream) {
     if (!aligned(p->weight, 16) || p->weight_row % 16 || p->weight_row < p->inputs || p->weight_row > (1 << 23)) return fail_msg(TAE_EINVAL, "int8_linear: weight rows start on 16-byte boundaries (quantize_int8 lays them so), at most 2^23 bytes apart");
     const size_t need = tae_int8_linear_workspace(p);
     if (!p->workspace || p->workspace_bytes < need || !aligned(p->workspace, 16)) return fail_msg(TAE_EINVAL, "int8_linear: the workspace is missing, misaligned or smaller than tae_int8_linear_workspace");
+    if (!elements_aligned(dtype_bytes(p->dtype), p->x, p->y) || !elements_aligned(4, p->weight_scale, p->bias)) return fail_msg(TAE_EINVAL, "int8_linear: a pointer is not aligned to its elements");
     const int64_t qr = q_stride(p->inputs);
     int8_t* q = (int8_t*)p->workspace;
     float* scale = (float*)(q + (size_t)p->rows * qr);

@@ -453,10 +453,13 @@ int tae_token_logprobs(const tae_logprobs_args* p, void* stream) {
     if (p->token_bytes != 4 && p->token_bytes != 8) return fail_msg(TAE_EINVAL, "token_logprobs: token_bytes must be 4 or 8");
     if (!p->logits || !p->tokens || !p->logp || !p->entropy) return fail_msg(TAE_EINVAL, "token_logprobs: logits, tokens, logp and entropy must not be NULL");
     if (p->top && (!p->top_ids || !p->top_logp)) return fail_msg(TAE_EINVAL, "token_logprobs: top needs top_ids and top_logp");
-    if (!aligned(p->logits, dtype_bytes(p->dtype)) || !aligned(p->tokens, p->token_bytes)) return fail_msg(TAE_EINVAL, "token_logprobs: a pointer is not aligned to its elements");
+    if (!elements_aligned(dtype_bytes(p->dtype), p->logits) || !elements_aligned(p->token_bytes, p->tokens) || !elements_aligned(4, p->logp, p->entropy, p->top_logp) ||
+        !elements_aligned(8, p->top_ids))
+        return fail_msg(TAE_EINVAL, "token_logprobs: a pointer is not aligned to its elements");
     LogprobsPlan s;
     const bool rows16 = aligned(p->logits, 16) && p->logits_row * (int64_t)dtype_bytes(p->dtype) % 16 == 0;
     if (!plan_logprobs(p, rows16, &s)) return fail_msg(TAE_EINVAL, "token_logprobs: bad sizes");
+    if ((int64_t)p->rows * s.parts > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "token_logprobs: too many rows for one call");
     if (s.bytes && (!p->workspace || p->workspace_bytes < s.bytes || !aligned(p->workspace, 16)))
         return fail_msg(TAE_EINVAL, "token_logprobs: the workspace is missing, misaligned or smaller than tae_token_logprobs_workspace");
     LogprobsArgs a{p->logits, p->tokens, p->logp, p->entropy, p->top_logp, p->top_ids, s.bytes ? (float*)p->workspace : nullptr,

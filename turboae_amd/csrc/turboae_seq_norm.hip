@@ -19,9 +19,14 @@ struct NormArgs {
     float eps, alpha;
 };
 
+// 1 - 2 / (1 + e^2g) of the magnitude, and next to 0, where that loses digits, the series up to g^9: what is left out is below 2^-26 of the value
+__device__ __forceinline__ float tanh_of(float g) {
+    const float s = g * g, series = g * __builtin_fmaf(s, __builtin_fmaf(s, __builtin_fmaf(s, __builtin_fmaf(s, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return fabsf(g) < 0.25f ? series : copysignf(1.0f - 2.0f * sigmoid(-2.0f * fabsf(g)), g);
+}
 __device__ __forceinline__ float gate_value(float g, int act) {
     switch (act) {
-        case TAE_ACT_TANH: return 2.0f * sigmoid(2.0f * g) - 1.0f;
+        case TAE_ACT_TANH: return tanh_of(g);
         case TAE_ACT_SIGMOID: return sigmoid(g);
         case TAE_ACT_SILU: return silu(g);
         default: return g;
@@ -57,17 +62,19 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
     const T* bl = (const T*)a.block + b * a.bl_b + t * a.bl_r;
     const T* ga = (const T*)a.gate + b * a.ga_b + t * a.ga_r;
     const float inv = 1.0f / (float)a.dim;
-    // all of the row is on its way before any of it is used; lanes behind the row repeat its last elements
+    // All of the row is on its way before any of it is used; lanes behind the row repeat its last elements.  Only with 32 elements for each
+    // of 1024 lanes (128 registers for each) the gate would not fit beside the rest: there it is loaded where it is used.
+    constexpr bool GATE_AHEAD = NV * V < 32;
     Raw<R, V> raw_r[NV];
-    Raw<T, V> raw_p[NV], raw_g[NV];
+    Raw<T, V> raw_p[NV], raw_g[GATE_AHEAD ? NV : 1];
 #pragma unroll
     for (int j = 0; j < NV; ++j) raw_r[j].from(rs + min((j * TPR + lane) * V, a.dim - V));
     if (a.block) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) raw_p[j].from(bl + min((j * TPR + lane) * V, a.dim - V));
-        if (a.gate) {
+        if (GATE_AHEAD && a.gate) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) raw_g[j].from(ga + min((j * TPR + lane) * V, a.dim - V));
+            for (int j = 0; j < NV; ++j) raw_g[GATE_AHEAD ? j : 0].from(ga + min((j * TPR + lane) * V, a.dim - V));
         }
     }
     float r[NV][V];
@@ -127,8 +134,10 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
                 for (int i = 0; i < V; ++i) f[i] *= w.v[i];
             }
             if (a.gate) {
+                Raw<T, V>& g = raw_g[GATE_AHEAD ? j : 0];
+                if (!GATE_AHEAD) g.from(ga + e);
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] *= gate_value(raw_g[j][i], a.gate_act);
+                for (int i = 0; i < V; ++i) f[i] *= gate_value(g[i], a.gate_act);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) p[j][i] = f[i];
@@ -218,7 +227,7 @@ extern "C" int tae_norm_residual(const tae_norm_args* p, void* stream) {
     if (p->residual_dtype != p->dtype && p->residual_dtype != TAE_DTYPE_F32) return fail_msg(TAE_EINVAL, "norm_residual: the residual has the block's type or fp32");
     if (p->batch < 1 || p->len < 1 || (int64_t)p->batch * p->len > INT32_MAX) return fail_msg(TAE_EINVAL, "norm_residual: batch and len must be >= 1, their product below 2^31");
     if (p->dim < 1 || p->dim > 32768) return fail_msg(TAE_EINVAL, "norm_residual: dim must be in 1..32768");
-    if (!(p->eps > 0.0f)) return fail_msg(TAE_EINVAL, "norm_residual: eps must be > 0");
+    if (!(p->eps >= 0x1p-126f)) return fail_msg(TAE_EINVAL, "norm_residual: eps must be > 0, and no subnormal number");
     if (p->gate_act != TAE_ACT_LINEAR && p->gate_act != TAE_ACT_TANH && p->gate_act != TAE_ACT_SIGMOID && p->gate_act != TAE_ACT_SILU)
         return fail_msg(TAE_EINVAL, "norm_residual: gate_act must be linear, tanh, sigmoid or silu");
     if (!p->residual) return fail_msg(TAE_EINVAL, "norm_residual: residual is NULL");
@@ -230,6 +239,9 @@ extern "C" int tae_norm_residual(const tae_norm_args* p, void* stream) {
     if (p->residual_out == p->residual && p->residual && (p->out_batch != p->residual_batch || p->out_row != p->residual_row))
         return fail_msg(TAE_EINVAL, "norm_residual: an in-place residual_out has the residual's strides");
     const size_t tb = dtype_bytes(p->dtype), rb = dtype_bytes(p->residual_dtype);
+    if (!elements_aligned(tb, p->block, p->gate, p->normed) || !elements_aligned(rb, p->residual, p->residual_out) ||
+        !elements_aligned(4, p->scale, p->post_weight, p->post_bias, p->pre_weight, p->pre_bias))
+        return fail_msg(TAE_EINVAL, "norm_residual: a pointer is not aligned to its elements");
     Width wt(tb), wr(rb), wf(4);
     wt.elements(p->dim).pointer(p->normed);
     if (p->block) wt.pointer(p->block).elements(p->block_batch).elements(p->block_row);

@@ -86,6 +86,7 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
     int group, piece;
     q.by_groups.split(id, rest, group);
     q.by_pieces.split(rest, b, piece);
+    if (ENDS && piece + 1 == q.pieces) return;   // nothing starts from there
     const int tid = threadIdx.x, ch = tid / P, p = tid % P;
     const int e0 = group * CW, e = e0 + ch, E = q.channels;
     const bool mine = e < E;
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            if constexpr (P >= 2) out[i] = dpp_add<kXor1>(out[i]);
+                            out[i] = dpp_add<kXor1>(out[i]);
                             if constexpr (P >= 4) out[i] = dpp_add<kXor2>(out[i]);
                         }
                         store<float, 4>(py, Pack<float, 4>{out[0], out[1], out[2], out[3]});
@@ -336,6 +337,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_lane_kernel(ScanArgs q) {
     int group, piece;
     q.by_groups.split(id, rest, group);
     q.by_pieces.split(rest, b, piece);
+    if (ENDS && piece + 1 == q.pieces) return;   // nothing starts from there
     const int lane = threadIdx.x & 63, p = lane % P, n0 = p * N, E = q.channels, e = group * CW + lane / P, ec = min(e, E - 1);
     const bool mine = e < E;
     const int n = q.lengths ? min(max(q.lengths[b], 0), q.len) : q.len;
@@ -531,7 +533,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs q, int
         for (int j = 0; j < A; ++j) {
             if (j0 + j < q.pieces) {
                 slot[(j0 + j) * step] = h;
-                h = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[j] * a2), h, part[j]);
+                // by its root twice: the whole factor may be infinite (a growing state) where its product is not; a state of 0 stays one
+                const float root = __builtin_amdgcn_exp2f(0.5f * sum[j] * a2);
+                h = h == 0.0f ? part[j] : __builtin_fmaf(root, root * h, part[j]);
             }
         }
     }
@@ -642,8 +646,8 @@ static bool plan_scan(const tae_scan_args* p, ScanPlan* out) {
     int padded = 4;
     while (padded < p->states) padded *= 2;
     double least = 0.0;
-    for (int form = 0; form < 8; ++form) {
-        const int tiled = form >= 3, lanes = tiled ? 1 << (form - 3) : 1 << form, per_lane = padded / lanes;
+    for (int form = 0; form < 7; ++form) {
+        const int tiled = form >= 3, lanes = tiled ? 2 << (form - 3) : 1 << form, per_lane = padded / lanes;
         if (lanes > padded || (tiled ? per_lane > 4 : per_lane < 4 || per_lane > 32)) continue;
         const int64_t groups = ceil_div(p->channels, tiled ? kScanThreads / lanes : 64 / lanes), waves = tiled ? 4 : 1;
         const double channel = tiled ? 1.0 / lanes : 1.0, across = tiled ? 18.0 : lanes > 1 ? 4.0 : 0.0;
@@ -721,7 +725,6 @@ static int launch_scan_plan(const ScanArgs& a, const ScanPlan& s, bool v, int ba
         case 404: return launch_lane<T, 4, 4>(a, batch, st);
         case 408: return launch_lane<T, 8, 4>(a, batch, st);
         case 416: return launch_lane<T, 16, 4>(a, batch, st);
-        case 10104: return launch_scan<T, 4, 1, 16>(a, v, batch, st);
         case 10202: return launch_scan<T, 2, 2, 16>(a, v, batch, st);
         case 10204: return launch_scan<T, 4, 2, 16>(a, v, batch, st);
         case 10401: return launch_scan<T, 1, 4, 32>(a, v, batch, st);
@@ -758,6 +761,8 @@ int tae_selective_scan(const tae_scan_args* p, void* stream) {
     if (p->batch < 1 || p->len < 1 || p->channels < 1) return fail_msg(TAE_EINVAL, "selective_scan: batch, len and channels must be >= 1");
     if (p->len > (1 << 30) || p->channels > (1 << 30)) return fail_msg(TAE_EINVAL, "selective_scan: len and channels must be at most 2^30");
     if (!p->x || !p->dt || !p->a || !p->b || !p->c || !p->y || !p->state_out) return fail_msg(TAE_EINVAL, "selective_scan: x, dt, a, b, c, y and state_out must not be NULL");
+    if (!elements_aligned(dtype_bytes(p->dtype), p->x, p->dt, p->b, p->c, p->z, p->y) || !elements_aligned(4, p->a, p->d, p->dt_bias, p->state, p->lengths, p->state_out))
+        return fail_msg(TAE_EINVAL, "selective_scan: a pointer is not aligned to its elements");
     ScanPlan s;
     if (!plan_scan(p, &s)) return fail_msg(TAE_EINVAL, "selective_scan: bad sizes");
     if (s.bytes && (!p->workspace || p->workspace_bytes < s.bytes || !aligned(p->workspace, 16)))

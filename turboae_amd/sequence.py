@@ -100,13 +100,20 @@ def _strides(t: Optional[torch.Tensor]) -> Tuple[int, int]:
     return t.stride()[:2] if t is not None and t.dim() == 3 else (0, 0)
 
 
-def _in_place_or_apart(name: str, source: Optional[torch.Tensor], out: torch.Tensor) -> None:
-    """An output may be its source itself; one that overlaps it in any other way is refused."""
-    if source is None or source.data_ptr() == out.data_ptr() and source.stride() == out.stride():
-        return
-    (a, m), (b, n) = ((t.data_ptr(), sum((s - 1) * d for s, d in zip(t.shape, t.stride())) * t.element_size() + t.element_size()) for t in (source, out))
-    if a < b + n and b < a + m:
-        raise ValueError(f"{name}: an output overlaps its source without being the same tensor")
+def _in_place_or_apart(name: str, out: torch.Tensor, same: Optional[torch.Tensor], *others: Optional[torch.Tensor]) -> None:
+    """An output may be `same` itself, element for element; one that overlaps an input in any other way is refused."""
+    b, n = out.data_ptr(), _extent(out)
+    for t in (same, *others):
+        if t is None or not t.is_cuda or t is same and t.data_ptr() == b and t.dtype is out.dtype and t.shape == out.shape and t.stride() == out.stride():
+            continue
+        a = t.data_ptr()
+        if a < b + n and b < a + _extent(t):
+            raise ValueError(f"{name}: an output overlaps an input without being the one that it may replace")
+
+
+def _extent(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    return (sum((s - 1) * d for s, d in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
@@ -126,7 +133,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     f32 = torch.float32
     y = torch.empty((B, L, E), dtype=c.dtype, device=c.device)
     if state_out is not None and K > 1:
-        _in_place_or_apart(c.name, state, state_out)
+        _in_place_or_apart(c.name, state_out, state, x, weight, bias, lengths)
     state_out = c.out(state_out, "state_out", (B, K - 1, E), c.dtype)
     args = _lib.TaeConvArgs(ctypes.sizeof(_lib.TaeConvArgs), _DTYPE[c.dtype], B, L, E, K, _ACT[act], 0, x.stride(0), x.stride(1),
                             c.tensor(x, "x", (B, L, E), c.dtype), c.tensor(weight, "weight", (E, K), f32, True), c.tensor(bias, "bias", (E,), f32, True),
@@ -155,7 +162,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     f32 = torch.float32
     y = torch.empty((b, L, E), dtype=c.dtype, device=c.device)
     if state_out is not None:
-        _in_place_or_apart(c.name, state, state_out)
+        _in_place_or_apart(c.name, state_out, state, x, dt, A, B, C, D, z, dt_bias, lengths)
     state_out = c.out(state_out, "state_out", (b, E, N), f32)
     args = _lib.TaeScanArgs(ctypes.sizeof(_lib.TaeScanArgs), _DTYPE[c.dtype], b, L, E, N, 1 if softplus else 0, 0,
                             *_strides(x), *_strides(dt), *_strides(B), *_strides(C), *_strides(z),
@@ -207,9 +214,10 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
         out = residual if block is None else torch.empty((B, L, D), dtype=residual.dtype, device=c.device)
     else:
         c.tensor(out, "residual_out", (B, L, D), residual.dtype)
-        if (L > 1 and out.stride(1) < D) or (B > 1 and out.stride(0) < (L - 1) * out.stride(1) + D):
+        (inner, n), (outer, m) = sorted(((out.stride(1), L), (out.stride(0), B))) if B > 1 and L > 1 else ((out.stride(1), L), (out.stride(0), B))
+        if (n > 1 and inner < D) or (m > 1 and outer < (n - 1) * inner + D):
             raise ValueError("norm_residual: rows of residual_out overlap")
-        _in_place_or_apart(c.name, residual, out)
+        _in_place_or_apart(c.name, out, residual, block, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     write = block is not None or (residual_out is not None and residual_out is not residual)
     normed = torch.empty((B, L, D), dtype=c.dtype, device=c.device) if pre_weight is not None else None
     vectors = [c.tensor(v, what, (D,), f32, True) for v, what in ((scale, "scale"), (post_weight, "post_weight"), (post_bias, "post_bias"),
