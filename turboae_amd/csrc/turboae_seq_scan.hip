@@ -451,10 +451,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_lane_kernel(ScanArgs q) {
 #pragma unroll
             for (int k = 0; k < G; ++k) h[k0 + k] = __builtin_fmaf(g[k], h[k0 + k], u[k]);
             if constexpr (!ENDS) {
-                float part[4] = {out[i], 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = 0; k < G; ++k) part[k & 3] = k < 4 && k > 0 ? h[k0 + k] * cv[at & 1][k] : __builtin_fmaf(h[k0 + k], cv[at & 1][k], part[k & 3]);
-                out[i] = (part[0] + part[1]) + (part[2] + part[3]);
+                for (int k = 0; k < G; ++k) out[i] = __builtin_fmaf(h[k0 + k], cv[at & 1][k], out[i]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }

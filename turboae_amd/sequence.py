@@ -38,14 +38,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 class _Call:
     """The checks that every tensor of a call goes through, against the first of them; a call of a single token costs little more."""
 
-    __slots__ = ("name", "device", "dtype", "grad")
+    __slots__ = ("name", "device", "dtype", "grad", "new")
 
     def __init__(self, name: str, first: torch.Tensor):
         if not isinstance(first, torch.Tensor) or not first.is_cuda:
             raise _lib.TurboAEError(f"{name}: needs tensors on a ROCm GPU device (no CPU fallback)")
         if first.dtype not in _DTYPE:
             raise ValueError(f"{name}: float32, float16 or bfloat16 wanted, got {first.dtype}")
-        self.name, self.device, self.dtype, self.grad = name, first.device, first.dtype, torch.is_grad_enabled()
+        self.name, self.device, self.dtype, self.grad, self.new = name, first.device, first.dtype, torch.is_grad_enabled(), first.new_empty
 
     def tensor(self, t: Optional[torch.Tensor], what: str, shape: Tuple[int, ...], dtype: torch.dtype, dense: bool = False) -> Optional[int]:
         """Address of a tensor after its checks (None for None): shape, type, device, adjacent last elements; dense: contiguous."""
@@ -65,7 +65,7 @@ class _Call:
     def out(self, t: Optional[torch.Tensor], what: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
         """A given output after its checks, or a new one."""
         if t is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return self.new(shape, dtype=dtype)
         self.tensor(t, what, shape, dtype, dense=True)
         return t
 
@@ -74,7 +74,7 @@ class _Call:
         n = size(ctypes.byref(args))
         if n == 0:
             return None
-        w = torch.empty(n, dtype=torch.uint8, device=self.device)
+        w = self.new(n, dtype=torch.uint8)
         args.workspace, args.workspace_bytes = w.data_ptr(), n
         return w
 
@@ -131,7 +131,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if not 1 <= K <= 8 or act not in ("linear", "silu"):
         raise ValueError(f"causal_conv: 1 to 8 taps and act 'linear' or 'silu' wanted, got {K} and {act!r}")
     f32 = torch.float32
-    y = torch.empty((B, L, E), dtype=c.dtype, device=c.device)
+    y = c.new((B, L, E), dtype=c.dtype)
     if state_out is not None and K > 1:
         _in_place_or_apart(c.name, state_out, state, x, weight, bias, lengths)
     state_out = c.out(state_out, "state_out", (B, K - 1, E), c.dtype)
@@ -160,7 +160,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         raise ValueError(f"selective_scan: A must have shape (channels, states) with 1 to 64 states, got {tuple(A.shape)}")
     N = A.shape[1]
     f32 = torch.float32
-    y = torch.empty((b, L, E), dtype=c.dtype, device=c.device)
+    y = c.new((b, L, E), dtype=c.dtype)
     if state_out is not None:
         _in_place_or_apart(c.name, state_out, state, x, dt, A, B, C, D, z, dt_bias, lengths)
     state_out = c.out(state_out, "state_out", (b, E, N), f32)
@@ -211,7 +211,7 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
         ga = gate.stride(0), gate.stride(1) if per_token else 0
     out = residual_out
     if out is None:
-        out = residual if block is None else torch.empty((B, L, D), dtype=residual.dtype, device=c.device)
+        out = residual if block is None else c.new((B, L, D), dtype=residual.dtype)
     else:
         c.tensor(out, "residual_out", (B, L, D), residual.dtype)
         (inner, n), (outer, m) = sorted(((out.stride(1), L), (out.stride(0), B))) if B > 1 and L > 1 else ((out.stride(1), L), (out.stride(0), B))
@@ -219,7 +219,7 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
             raise ValueError("norm_residual: rows of residual_out overlap")
         _in_place_or_apart(c.name, out, residual, block, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     write = block is not None or (residual_out is not None and residual_out is not residual)
-    normed = torch.empty((B, L, D), dtype=c.dtype, device=c.device) if pre_weight is not None else None
+    normed = c.new((B, L, D), dtype=c.dtype) if pre_weight is not None else None
     vectors = [c.tensor(v, what, (D,), f32, True) for v, what in ((scale, "scale"), (post_weight, "post_weight"), (post_bias, "post_bias"),
                                                                   (pre_weight, "pre_weight"), (pre_bias, "pre_bias"))]
     args = _lib.TaeNormArgs(ctypes.sizeof(_lib.TaeNormArgs), _DTYPE[c.dtype], _DTYPE[residual.dtype], B, L, D, 1 if center else 0, _ACT[gate_act], eps, alpha,
@@ -240,8 +240,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     R, K = x.shape
     address = c.tensor(x, "x", (R, K), c.dtype)
     step = -(-K // 64) * 64
-    q = torch.empty((R, step), dtype=torch.int8, device=c.device)
-    scale = torch.empty(R, dtype=torch.float32, device=c.device)
+    q = c.new((R, step), dtype=torch.int8)
+    scale = c.new(R, dtype=torch.float32)
     c.run(_lib.load().tae_quantize_int8, _DTYPE[c.dtype], address, x.stride(0), R, K, q.data_ptr(), step, scale.data_ptr())
     return q[:, :K], scale
 
@@ -266,7 +266,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if weight.storage_offset() + (N - 1) * step + -(-K // 16) * 16 > weight.untyped_storage().nbytes():
         raise ValueError("int8_linear: the last weight row must reach to its next 16-byte boundary (quantize_int8 lays them so)")
     f32 = torch.float32
-    y = torch.empty((*x.shape[:-1], N), dtype=c.dtype, device=c.device)
+    y = c.new((*x.shape[:-1], N), dtype=c.dtype)
     args = _lib.TaeInt8Args(ctypes.sizeof(_lib.TaeInt8Args), _DTYPE[c.dtype], M, K, N, 0, rows.stride(0), step, rows.data_ptr(), address,
                             c.tensor(weight_scale, "weight_scale", (N,), f32, True), c.tensor(bias, "bias", (N,), f32, True), y.data_ptr(), None, 0)
     lib = _lib.load()
@@ -291,10 +291,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     flat = logits if logits.dim() == 2 else logits.reshape(-1, V)
     R = flat.shape[0]
     shape = tuple(tokens.shape)
-    logp = torch.empty(shape, dtype=torch.float32, device=c.device)
-    entropy = torch.empty(shape, dtype=torch.float32, device=c.device)
-    ids = torch.empty((*shape, top), dtype=torch.int64, device=c.device) if top else None
-    top_logp = torch.empty((*shape, top), dtype=torch.float32, device=c.device) if top else None
+    logp = c.new(shape, dtype=torch.float32)
+    entropy = c.new(shape, dtype=torch.float32)
+    ids = c.new((*shape, top), dtype=torch.int64) if top else None
+    top_logp = c.new((*shape, top), dtype=torch.float32) if top else None
     args = _lib.TaeLogprobsArgs(ctypes.sizeof(_lib.TaeLogprobsArgs), _DTYPE[c.dtype], 8 if tokens.dtype == torch.int64 else 4, R, V, top, flat.stride(0),
                                 c.tensor(flat, "logits", (R, V), c.dtype), c.tensor(tokens, "tokens", shape, tokens.dtype, True), logp.data_ptr(), entropy.data_ptr(),
                                 ids.data_ptr() if top else None, top_logp.data_ptr() if top else None, None, 0)
