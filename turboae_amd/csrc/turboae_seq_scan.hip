@@ -320,18 +320,27 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
 
 // P = 1, 2 or 4 adjacent lanes own a channel, each N of its states (n = p N + k); a wave walks the positions of its piece by itself.  B[t] and
 // C[t] are the same for all channels and come from LDS, so that a state costs five instructions (two products, exp, two fused) and only one
-// sum over P lanes crosses them; steps and gates are worked out by each of the P.  All loads
-// are kAhead positions ahead; each wave has LDS of its own, so no barrier is needed; four of
-// them make a workgroup only because its waves are dealt out evenly over a CU's SIMDs.
-constexpr int kAhead = 8;
+// sum over P lanes crosses them; steps and gates are worked out by each of the P.  All loads are kAhead positions ahead; each wave has LDS of
+// its own, so no barrier is needed.
+//
+// Bound by issuing: 119 vector instructions (20 of them exp, log and rcp at half rate) for each position of 64 channels with 16 states.
+// Eight waves make a workgroup so that they are dealt out evenly over a CU's SIMDs, two each (waves w and w + 4), and know of each other:
+// left alone the older of two gets most of the issue slots and the younger runs by itself at the end, at half the rate (61 and 83 us of a
+// wave's life where both should take 72).  So whichever has more positions left goes first.  Measured, bf16, 4096 positions x 4096 channels
+// x 16 states in 32 pieces: 90 us, ends pass 65 (four waves, no priorities: 90 and 68); fp32, 500 x 100 x 200 x 16: 48 (57).  More pieces,
+// so more waves, are no faster (48: 94 + 69, 64: 92 + 71), fewer are slower (16: 129 + 84), and so are two lanes for a channel (116 + 75).
+constexpr int kAhead = 8, kLaneWaves = 8;
 
 template <class T, int N, int P, bool ENDS>
-__global__ __launch_bounds__(kScanThreads) void scan_lane_kernel(ScanArgs q) {
+__global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) {
     constexpr int NP = N * P, W = ENDS ? NP : 2 * NP, CW = 64 / P, RB = (kAhead * W + 63) / 64;       // values of B (and C) for each position; loads of each lane
-    __shared__ alignas(16) float lds[kScanThreads / 64][2][kAhead * W];
+    __shared__ alignas(16) float lds[kLaneWaves][2][kAhead * W];
+    __shared__ int left[kLaneWaves];    // positions; read without a barrier, for priorities only
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto report = [&](int positions) { if ((threadIdx.x & 63) == 0) __hip_atomic_store(&left[wave], positions, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
+    report(0);
     float(*rows)[kAhead * W] = lds[wave];
-    const int64_t id = block_index() * (kScanThreads / 64) + wave;
+    const int64_t id = block_index() * (kLaneWaves) + wave;
     if (id >= q.blocks) return;
     int64_t rest, b;
     int group, piece;
@@ -481,6 +490,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_lane_kernel(ScanArgs q) {
     int t0 = begin;
     for (; t0 + kAhead <= stop; t0 += kAhead) {
         const bool more = t0 + kAhead < stop;
+        report(stop - t0);
+        if (__builtin_amdgcn_readfirstlane(__hip_atomic_load(&left[wave ^ 4], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) < stop - t0) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
         if (more) fetch(next, t0 + kAhead);
         block(t0, kAhead, buf);
         if (more) stage(next, buf ^ 1);
@@ -699,12 +711,12 @@ static int launch_scan(const ScanArgs& a, bool vector, int64_t batch, hipStream_
 
 template <class T, int N, int P>
 static int launch_lane(const ScanArgs& a, int64_t batch, hipStream_t st) {
-    const dim3 grid = grid_of(ceil_div(a.blocks, kScanThreads / 64));
+    const dim3 grid = grid_of(ceil_div(a.blocks, kLaneWaves)), block(kLaneWaves * 64);
     if (a.pieces > 1) {
-        hipLaunchKernelGGL((scan_lane_kernel<T, N, P, true>), grid, dim3(kScanThreads), 0, st, a);
+        hipLaunchKernelGGL((scan_lane_kernel<T, N, P, true>), grid, block, 0, st, a);
         launch_join(a, batch, st);
     }
-    hipLaunchKernelGGL((scan_lane_kernel<T, N, P, false>), grid, dim3(kScanThreads), 0, st, a);
+    hipLaunchKernelGGL((scan_lane_kernel<T, N, P, false>), grid, block, 0, st, a);
     return TAE_OK;
 }
 
