@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <type_traits>
 
 #include "../../include/turboae_hip.h"
 

@@ -128,6 +128,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
     uint32_t w[G][D];
     auto value = [&](int g, int i) -> float {
         if constexpr (V == 1 || sizeof(T) == 4) return __uint_as_float(w[g][i]);
+        // by bits: of a conversion the compiler would make bf16 maxima, back and forth
+        else if constexpr (std::is_same_v<T, bf16>) return __uint_as_float(i & 1 ? w[g][i / 2] & 0xFFFF0000u : w[g][i / 2] << 16);
         else return (float)__builtin_bit_cast(T, (uint16_t)(i & 1 ? w[g][i / 2] >> 16 : w[g][i / 2] & 0xFFFFu));
     };
     auto again = [&]() {
@@ -208,18 +210,25 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
             if (a.top && own >= bound && slot < 64) tops[slot] = own;
         }
     }
-    // e^(x - m) = 2^((x - m) log2 e), the difference first: one fused instruction less would lose it next to a maximum like the type's lowest
-    // value; -inf (and what is far below m) is taken at 2^-1000 = 0, so that 0 times its distance is 0
-    const float base = m == kNegInf ? 0.0f : m;
+    // e^(x - m) = 2^(x log2 e - c), c = m log2 e rounded, with one fused product; by how much c was rounded is known exactly (`off`) and put
+    // right in the sums.  Where that could be much (a maximum like the type's lowest value) the difference comes first.  -inf, and what is
+    // far below m, is taken at 2^-1000 = 0, so that 0 times its distance is 0.
+    const float base = m == kNegInf ? 0.0f : m, c = base * kLog2e;
+    const bool near = fabsf(base) < 0x1p20f;
+    const float off = near ? __builtin_fmaf(base, kLog2e, -c) : 0.0f;
     float s = 0.0f, t = 0.0f;
+    auto sums = [&](auto&& distance) {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float d = fmaxf((value(g, i) - base) * kLog2e, -1000.0f), e = __builtin_amdgcn_exp2f(d);
-            s += e;
-            t = __builtin_fmaf(d, e, t);
-        }
+            for (int i = 0; i < V; ++i) {
+                const float d = fmaxf(distance(value(g, i)), -1000.0f), e = __builtin_amdgcn_exp2f(d);
+                s += e;
+                t = __builtin_fmaf(d, e, t);
+            }
+    };
+    if (near) sums([&](float x) { return __builtin_fmaf(x, kLog2e, -c); });
+    else sums([&](float x) { return (x - base) * kLog2e; });
     again();
     s = lanes_sum<WW>(s);
     t = lanes_sum<WW>(t);
@@ -230,6 +239,9 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) { s += lds_f[i][1]; t += lds_f[i][2]; }
     }
+    const float back = __builtin_amdgcn_exp2f(-off);
+    s *= back;
+    t = __builtin_fmaf(t, back, -off * s);
     const Stats st{m, s, t * kLn2};
     const bool none = m != m || m == __builtin_inff();
     const float log_s = __builtin_amdgcn_logf(s) * kLn2;
@@ -259,8 +271,9 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
             if (!__any(!(of[g] < least))) continue;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const int at = place(g) + i;
                 const float v = value(g, i);
+                if (!__any(!(v < least))) continue;
+                const int at = place(g) + i;
                 const bool yes = !(v < least) && at >= lo && at < hi;
                 const u64 set = __ballot(yes);
                 const uint32_t slot = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
