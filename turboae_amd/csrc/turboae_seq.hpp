@@ -31,6 +31,16 @@ __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cas
 template <class T, int V>
 __device__ __forceinline__ void store(T* p, const Pack<T, V>& a) { *reinterpret_cast<Pack<T, V>*>(p) = a; }
 
+// The same from and to an address that is aligned to its elements only
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load_any(const T* p) {
+    Pack<T, V> a;
+    __builtin_memcpy(&a, p, sizeof(a));
+    return a;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_any(T* p, const Pack<T, V>& a) { __builtin_memcpy(p, &a, sizeof(a)); }
+
 // V adjacent elements as they were loaded, in whole registers: an element is taken out when it is used, so that a load stays in flight until
 // then and 16-bit elements need no registers of their own.
 template <class T, int V>

@@ -41,7 +41,8 @@ __device__ __forceinline__ Pack<int8_t, V> whole_numbers(const Pack<T, V>& p, fl
     return o;
 }
 
-// One workgroup for each row, which stays in registers (KEEP groups of V for each lane) or, with KEEP = 0, is read twice.
+// One workgroup for each row, which stays in registers (KEEP groups of V for each lane; a row holds one at least) or, with KEEP = 0, is read
+// twice.  Rows may start on any element: wide loads need no more here.
 template <class T, int V, int KEEP>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     __shared__ float lds[4];
@@ -59,14 +60,26 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
             most = fmaxf(most, v);
         }
     };
+    auto edge = [&](int e) {                     // the last group of a row, zeros behind it
+        Pack<T, V> p;
+#pragma unroll
+        for (int i = 0; i < V; ++i) p.v[i] = e + i < a.cols ? x[e + i] : (T)0.0f;
+        return p;
+    };
     Pack<T, V> kept[KEEP > 0 ? KEEP : 1];
     if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int j = 0; j < KEEP; ++j) kept[j] = load<T, V>(x + min((j * 256 + tid) * V, a.cols - V));
+        for (int j = 0; j < KEEP; ++j) kept[j] = load_any<T, V>(x + min((j * 256 + tid) * V, a.cols - V));
 #pragma unroll
-        for (int j = 0; j < KEEP; ++j) look(kept[j]);
+        for (int j = 0; j < KEEP; ++j) {
+            const int e = (j * 256 + tid) * V;
+            if (e < a.cols && e + V > a.cols) kept[j] = edge(e);
+            look(kept[j]);
+        }
     } else {
-        for (int e = tid * V; e < a.cols; e += 256 * V) look(load<T, V>(x + e));
+        int e = tid * V;
+        for (; e + V <= a.cols; e += 256 * V) look(load_any<T, V>(x + e));
+        if (e < a.cols) look(edge(e));
     }
     if (__any(bad)) most = __builtin_inff();
     most = lanes_max<64>(most);
@@ -87,20 +100,22 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
         }
         for (int e = (KEEP * 256 + tid) * V; e < a.q_r; e += 256 * V) store<int8_t, V>(q + e, zeros);
     } else {
-        for (int e = tid * V; e < a.q_r; e += 256 * V) store<int8_t, V>(q + e, fine && e < a.cols ? whole_numbers<T, V>(load<T, V>(x + e), by, reciprocal) : zeros);
+        int e = tid * V;
+        if (fine) {
+            for (; e + V <= a.cols; e += 256 * V) store<int8_t, V>(q + e, whole_numbers<T, V>(load_any<T, V>(x + e), by, reciprocal));
+            if (e < a.cols) store<int8_t, V>(q + e, whole_numbers<T, V>(edge(e), by, reciprocal)), e += 256 * V;
+        }
+        for (; e < a.q_r; e += 256 * V) store<int8_t, V>(q + e, zeros);
     }
 }
 
 template <class T>
 static void launch_quantize(const QuantArgs& a, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    Width w(sizeof(T));
-    w.elements(a.cols).elements(a.x_r).pointer(a.x);
     const dim3 grid = grid_of(a.rows), block(256);
-    if (!w.fits(16)) hipLaunchKernelGGL((quantize_int8_kernel<T, 1, 0>), grid, block, 0, st, a);
-    else if (a.cols <= 256 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 1>), grid, block, 0, st, a);
-    else if (a.cols <= 512 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 2>), grid, block, 0, st, a);
-    else if (a.cols <= 1024 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 4>), grid, block, 0, st, a);
+    if (a.cols >= V && a.cols <= 256 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 1>), grid, block, 0, st, a);
+    else if (a.cols >= V && a.cols <= 512 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 2>), grid, block, 0, st, a);
+    else if (a.cols >= V && a.cols <= 1024 * V) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 4>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((quantize_int8_kernel<T, V, 0>), grid, block, 0, st, a);
 }
 
@@ -255,6 +270,8 @@ __global__ __launch_bounds__(WM * WN * 64, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
                 T* y = (T*)a.y + (int64_t)m * a.n + n;
                 if (whole) {
                     if (m < a.m) store_once(y, out);
+                } else if (n + 16 <= a.n) {
+                    if (m < a.m) store_any(y, out);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 16; ++c)
@@ -382,8 +399,8 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
         if (m >= a.m || n >= a.n) continue;
         const Pack<T, 4> out = Outputs<T, 4>(a, n).row({sum[0], sum[1], sum[2], sum[3]}, a.scale[m]);
         T* y = (T*)a.y + (int64_t)m * a.n + n;
-        if (a.wide) {                            // outputs come in whole groups of four
-            store<T, 4>(y, out);
+        if (n + 4 <= a.n) {
+            store_any(y, out);
         } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -415,24 +432,34 @@ static hipError_t launch_few(Int8Args a, hipStream_t st) {
     return hipSuccess;
 }
 
-// Which form: measured whole calls in bf16, in us -
-//     4096 inputs and outputs, rows       64  128  256  512  1024  2048  3000  4096
-//     few, 32 x 32 a workgroup            15   22   37   67   126   243
-//     few, 64 x 32                        18   19   30   54   100   190
-//     tiles of 128 x 128, four buffers    23   23   24   27    30    51    72    98
-//     the same, two buffers, two for a CU 25   26   27   30    34    47    67    91
-//     tiles of 256 x 256                                             57    63    83
-//     8000 rows, 4000 outputs, inputs    200  500  1000  2000
-//     128 x 128, four / two buffers    41/35  53/47  70/63  107/96         256 x 256   57  65  78  101
-// and with 256 rows, 16000 inputs and 512 outputs, where tiles are too few for the CUs, few 43, tiles of 128 x 128 71.
+// Which form.  Up to 256 tiles of 128 x 128 the cheapest by what whole calls measured in bf16, in us, kk = inputs / 4096 and r rounds of 256
+// workgroups (1 at least):
+//     few, 16 x 16 a workgroup   5.2 + 1.2 kk + r max(3.5, 3.7 kk)        few, 64 x 32   6.0 + 1.2 kk + r max(4.2, 11.4 kk)
+//     few, 32 x 32               5.2 + 1.2 kk + r max(3.0, 7.2 kk)        tiles          8.0 + 15.6 kk
+// off by a tenth at most from 512 to 16384 inputs, 64 to 16384 outputs and 16 to 512 rows.  Among them, with 4096 outputs:
+//     4096 inputs, rows    16   32   64  128  256  512          16384 inputs, rows   16   32   64  128  256  512
+//     16 x 16              10   14   22   38   69  131                               27   42   71  127  236  458
+//     32 x 32              12   14   14   22   36   66                               38   41   42   70  126  239
+//     64 x 32              14   16   18   19   30   53                               43   48   56   57  100  185
+//     tiles                22   23   22   23   24   26                               71   71   71   71   72   76
+// More tiles:
+//     4096 inputs and outputs, rows                        1024  2048  3000  4096          8000 rows, 4000 outputs, inputs  200  500 1000 2000
+//     128 x 128, four buffers                                30    51    72    98                                            41   53   70  107
+//     the same, two buffers, two workgroups for a CU         34    46    67    91                                            35   47   63   96
+//     256 x 256                                                    57    63    83                                            57   65   78  101
 template <class T>
 static hipError_t launch_int8(const Int8Args& a, hipStream_t st) {
-    if (a.m <= 16) return launch_few<T, 1, 1, 8>(a, st);
     const int64_t large = ceil_div(a.m, 256) * ceil_div(a.n, 256), small = ceil_div(a.m, 128) * ceil_div(a.n, 128);
-    if (a.m <= 64 || (small < 64 && a.k >= 4096)) return launch_few<T, 2, 2, 4>(a, st);
-    if (a.m <= 128) return launch_few<T, 4, 2, 4>(a, st);
     if (large >= 192 && a.k >= 4096) return launch_tiles<T, 256, 256, 2, 4, 2>(a, st);
-    return small <= 256 ? launch_tiles<T, 128, 128, 2, 2, 4>(a, st) : launch_tiles<T, 128, 128, 2, 2, 2>(a, st);
+    if (small > 256) return launch_tiles<T, 128, 128, 2, 2, 2>(a, st);
+    const double kk = a.k / 4096.0;
+    auto rounds = [&](int rows, int outputs) { return std::max(1.0, ceil_div(a.m, rows) * ceil_div(a.n, outputs) / 256.0); };
+    const double by16 = 5.2 + 1.2 * kk + rounds(16, 16) * std::max(3.5, 3.7 * kk), by32 = 5.2 + 1.2 * kk + rounds(32, 32) * std::max(3.0, 7.2 * kk);
+    const double by64 = 6.0 + 1.2 * kk + rounds(64, 32) * std::max(4.2, 11.4 * kk), tiles = 8.0 + 15.6 * kk, least = std::min({by16, by32, by64, tiles});
+    if (least == by16) return launch_few<T, 1, 1, 8>(a, st);
+    if (least == by32) return launch_few<T, 2, 2, 4>(a, st);
+    if (least == by64) return launch_few<T, 4, 2, 4>(a, st);
+    return launch_tiles<T, 128, 128, 2, 2, 4>(a, st);
 }
 
 // Rows 1024 bytes and multiples apart would send a slab's lines of all rows to few channels of L2.

@@ -342,7 +342,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
 }
 
 // Joins the parts of a row, one workgroup for each: the statistics by rescaling, the sorted lists of alternatives by counting larger keys.
-// With as many parts as alternatives, what is below the top-th largest first key is left out beforehand.
+// What cannot be among them is left out beforehand: with j = ceil(top / parts), r = ceil(top / j), the r-th largest of the lists' j-th keys has
+// j r >= top keys at or above it.
 template <class T>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobsArgs a) {
     extern __shared__ u64 lists[];               // parts x top
@@ -372,16 +373,15 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobsArgs a) {
         finish_row(a, row, st, log_s, none, xt, token);
     }
     if (!a.top) return;
-    if (a.parts >= a.top) {
-        for (int p = tid; p < a.parts; p += 256) {
-            const u64 k = lists[p * a.top];
-            int rank = 0;
-            for (int i = 0; i < a.parts; ++i) rank += lists[i * a.top] > k;
-            if (rank == a.top - 1 && k) bound = k;
-        }
-        __syncthreads();
+    const int jth = (a.top + a.parts - 1) / a.parts, rth = (a.top + jth - 1) / jth;
+    for (int p = tid; p < a.parts; p += 256) {
+        const u64 k = lists[p * a.top + jth - 1];
+        int rank = 0;
+        for (int i = 0; i < a.parts; ++i) rank += lists[i * a.top + jth - 1] > k;
+        if (rank == rth - 1 && k) bound = k;
     }
-    // at most top lists of top keys each are left
+    __syncthreads();
+    // at most rth lists of top keys each and jth - 1 of the others are left: 1024 at the most, with top = 32
     for (int i = tid; i < all; i += 256) {
         const u64 k = lists[i];
         if (k >= bound) found[atomicAdd(&count, 1u)] = k;

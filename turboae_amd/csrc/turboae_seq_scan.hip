@@ -78,6 +78,7 @@ template <class T, int S, int P, int TT, int V, bool ENDS>
 __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q) {
     constexpr int CW = kScanThreads / P, N = S * P, DS = TT + 4;
     constexpr int R = TT * CW / 4 / kScanThreads, RB = (TT * N + kScanThreads - 1) / kScanThreads;      // groups of four, elements for each thread
+    static_assert(P == 4 || P == 8 || P == 16, "sums over lanes");
     static_assert(R >= 1 && TT * CW % (4 * kScanThreads) == 0, "a tile is whole groups of four for every thread");
     __shared__ float sd[2][CW * DS], sx[2][CW * DS], sb[2][N * DS], sc[ENDS ? 1 : 2][ENDS ? 4 : N * DS], sy[ENDS ? 1 : 2][ENDS ? 4 : CW * DS];
     const int64_t id = block_index();
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             out[i] = dpp_add<kXor1>(out[i]);
-                            if constexpr (P >= 4) out[i] = dpp_add<kXor2>(out[i]);
+                            out[i] = dpp_add<kXor2>(out[i]);
                         }
                         store<float, 4>(py, Pack<float, 4>{out[0], out[1], out[2], out[3]});
                     }
@@ -318,22 +319,21 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
     }
 }
 
-// P = 1, 2 or 4 adjacent lanes own a channel, each N of its states (n = p N + k); a wave walks the positions of its piece by itself.  B[t] and
-// C[t] are the same for all channels and come from LDS, so that a state costs five instructions (two products, exp, two fused) and only one
-// sum over P lanes crosses them; steps and gates are worked out by each of the P.  All loads are kAhead positions ahead; each wave has LDS of
-// its own, so no barrier is needed.
+// A lane owns a channel with its N states; a wave walks the positions of its piece by itself.  B[t] and C[t] are the same for all channels and
+// come from LDS, so that a state costs five instructions (two products, exp, two fused) and no sum crosses lanes.  All loads are kAhead
+// positions ahead; each wave has LDS of its own, so no barrier is needed.
 //
 // Bound by issuing: 119 vector instructions (20 of them exp, log and rcp at half rate) for each position of 64 channels with 16 states.
 // Eight waves make a workgroup so that they are dealt out evenly over a CU's SIMDs, two each (waves w and w + 4), and know of each other:
 // left alone the older of two gets most of the issue slots and the younger runs by itself at the end, at half the rate (61 and 83 us of a
 // wave's life where both should take 72).  So whichever has more positions left goes first.  Measured, bf16, 4096 positions x 4096 channels
 // x 16 states in 32 pieces: 90 us, ends pass 65 (four waves, no priorities: 90 and 68); fp32, 500 x 100 x 200 x 16: 48 (57).  More pieces,
-// so more waves, are no faster (48: 94 + 69, 64: 92 + 71), fewer are slower (16: 129 + 84), and so are two lanes for a channel (116 + 75).
+// so more waves, are no faster (48: 94 + 69, 64: 92 + 71), fewer are slower (16: 129 + 84).
 constexpr int kAhead = 8, kLaneWaves = 8;
 
-template <class T, int N, int P, bool ENDS>
+template <class T, int N, bool ENDS>
 __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) {
-    constexpr int NP = N * P, W = ENDS ? NP : 2 * NP, CW = 64 / P, RB = (kAhead * W + 63) / 64;       // values of B (and C) for each position; loads of each lane
+    constexpr int W = ENDS ? N : 2 * N, RB = (kAhead * W + 63) / 64;       // values of B (and C) for each position; loads of each lane
     __shared__ alignas(16) float lds[kLaneWaves][2][kAhead * W];
     __shared__ int left[kLaneWaves];    // positions; read without a barrier, for priorities only
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
     q.by_groups.split(id, rest, group);
     q.by_pieces.split(rest, b, piece);
     if (ENDS && piece + 1 == q.pieces) return;   // nothing starts from there
-    const int lane = threadIdx.x & 63, p = lane % P, n0 = p * N, E = q.channels, e = group * CW + lane / P, ec = min(e, E - 1);
+    const int lane = threadIdx.x & 63, E = q.channels, e = group * 64 + lane, ec = min(e, E - 1);
     const bool mine = e < E;
     const int n = q.lengths ? min(max(q.lengths[b], 0), q.len) : q.len;
     const int begin = piece * q.piece_len, end = min(begin + q.piece_len, q.len), stop = min(end, n);
@@ -357,8 +357,8 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
     const float* kept = q.pieces > 1 ? q.states + ((b * (q.pieces + 1) + piece) * q.n) * E + ec : nullptr;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int kc = min(n0 + k, q.n - 1);
-        const bool real = n0 + k < q.n;
+        const int kc = min(k, q.n - 1);
+        const bool real = k < q.n;
         a2[k] = real ? q.a[(int64_t)ec * q.n + kc] * kLog2e : 0.0f;
         h[k] = 0.0f;
         if (start) h[k] = real ? start[(b * E + ec) * q.n + kc] : 0.0f;
@@ -392,9 +392,9 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
         }
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
-            const int i = j * 64 + lane, k = i % NP;
+            const int i = j * 64 + lane, k = i % N;
             const int64_t t = min(t0 + min(i / W, kAhead - 1), stop - 1);
-            const T* row = !ENDS && i / NP % 2 ? cm + t * q.c_r : bm + t * q.b_r;
+            const T* row = !ENDS && i / N % 2 ? cm + t * q.c_r : bm + t * q.b_r;
             r.bc[j].from(row, k, q.n);
         }
     };
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
             const int i = j * 64 + lane;
-            if (kAhead * W % 64 == 0 || i < kAhead * W) rows[buf][i] = i % NP < q.n ? r.bc[j][0] : 0.0f;
+            if (kAhead * W % 64 == 0 || i < kAhead * W) rows[buf][i] = i % N < q.n ? r.bc[j][0] : 0.0f;
         }
     };
     Raw now, next;
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
         for (int i = 0; i < kAhead; ++i) {
             const float xv = now.x[i][0];
             dx[i] = d[i] * xv;
-            out[i] = P == 1 || p == 0 ? dcoef * xv : 0.0f;
+            out[i] = dcoef * xv;
             if constexpr (ENDS) sum += i < count ? d[i] : 0.0f;
         }
         // G states at a time: their products, exps, products and fused adds each as G instructions in a row, so that none waits for the one in
@@ -429,14 +429,14 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
         constexpr int G = N < 8 ? N : 8, GROUPS = N / G;
         float bv[2][G], cv[2][G];
         auto read = [&](int at, int to) {
-            const float* row = &rows[buf][at / GROUPS * W + n0 + at % GROUPS * G];
+            const float* row = &rows[buf][at / GROUPS * W + at % GROUPS * G];
 #pragma unroll
             for (int k = 0; k < G; k += 4) {
                 const Pack<float, 4> p = load<float, 4>(row + k);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) bv[to][k + c] = p.v[c];
                 if constexpr (!ENDS) {
-                    const Pack<float, 4> r = load<float, 4>(row + NP + k);
+                    const Pack<float, 4> r = load<float, 4>(row + N + k);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) cv[to][k + c] = r.v[c];
                 }
@@ -466,16 +466,11 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (!ENDS) {
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                if constexpr (P >= 2) out[i] = dpp_add<kXor1>(out[i]);
-                if constexpr (P >= 4) out[i] = dpp_add<kXor2>(out[i]);
-            }
             if (q.gate) {
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) out[i] *= silu(now.z[i][0]);
             }
-            if (mine && p == 0) {
+            if (mine) {
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
                     if (i < count) y[(int64_t)(t0 + i) * E + e] = (T)out[i];
@@ -505,14 +500,14 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
         float* to = q.states + ((b * (q.pieces + 1) + piece + 1) * q.n) * E + e;
 #pragma unroll
         for (int k = 0; k < N; ++k)
-            if (n0 + k < q.n) to[(int64_t)(n0 + k) * E] = h[k];
-        if (p == 0) q.steps[(b * q.pieces + piece) * E + e] = sum;
+            if (k < q.n) to[(int64_t)k * E] = h[k];
+        q.steps[(b * q.pieces + piece) * E + e] = sum;
     } else {
-        for (int t = max(begin, stop) + p; t < end; t += P) y[(int64_t)t * E + e] = (T)0.0f;
+        for (int t = max(begin, stop); t < end; ++t) y[(int64_t)t * E + e] = (T)0.0f;
         if (piece == last_piece) {
 #pragma unroll
             for (int k = 0; k < N; ++k)
-                if (n0 + k < q.n) q.state_out[(b * E + e) * q.n + n0 + k] = h[k];
+                if (k < q.n) q.state_out[(b * E + e) * q.n + k] = h[k];
         }
     }
 }
@@ -636,46 +631,56 @@ static int launch_steps(const ScanArgs& a, int batch, hipStream_t st) {
     return batch >= 4 && (int64_t)a.channels * a.n / V * batch >= 4 * 512 * kScanThreads ? launch_step<T, V, 4>(a, batch, st) : launch_step<T, V, 1>(a, batch, st);
 }
 
-// How a call is cut: P lanes for a channel, each with S states, by scan_lane_kernel or (tiled) selective_scan_kernel, and pieces.
+// How a call is cut: lanes for a channel, each with per_lane states, and pieces along the positions.
 struct ScanPlan {
-    int lanes = 1, per_lane = 1, tiled = 0, groups = 1, pieces = 1, piece_len = 0;
+    int lanes = 1, per_lane = 1, groups = 1, pieces = 1, piece_len = 0;
     size_t steps_bytes = 0, bytes = 0;
 };
 
 constexpr int kPieceUnit = 64;                   // pieces are whole tiles
 
-// Few channels leave SIMDs empty: then fewer states for each lane, or pieces along the positions, which cost a second pass (ENDS).  The
-// choice is the cheapest by the time that a wave takes for one position, times the positions and the waves that a SIMD (1024 of them) runs.
-// Measured: a vector instruction issues every 2.0 ns, an exp every 4.4, and a single wave reaches half of that, so one wave takes as long as
-// two.  A state takes four instructions and an exp, 12.4 ns (three in the ends pass, 10.4); the softplus, gate and D of a channel 55 ns (ends
-// pass: 30), by every lane of a channel in scan_lane_kernel, shared by its P lanes in the tiled one, which adds about 18 for sums over lanes,
-// LDS and barriers.
+// The ways to share a channel's states (4, 8, 16, 32 or 64 with those filled up) among lanes: by scan_lane_kernel with one lane, else by
+// selective_scan_kernel.  ns: what a wave takes for a position, with other waves on its SIMD; alone: the number of waves whose time one by
+// itself takes; start: us before a round of waves is under way.  Measured over lengths from 32 to 8192 and 128 to 131072 channels of all
+// sequences together, in bf16 with gate; what follows from them is within 16 % of the best of these ways and pieces.
+//     us, pieces in (); batch x len x channels x states      1 lane      4 lanes     8 lanes     16 lanes
+//     1 x 4096 x 4096 x 16                                   146 (32)                136 (32)    163 (16)
+//     8 x 2048 x 1024 x 16                                   147 (16)                131 (8)     127 (1)
+//     1 x 2048 x 512 x 16                                     78 (32)                 24 (32)     26 (16)
+//     64 x 256 x 256 x 16                                     82 (4)                  31 (1)      37 (1)
+//     500 x 100 x 200 x 16                                    69 (1)                  71 (1)      91 (1)
+//     2 x 2048 x 2048 x 32                                                           128 (8)     122 (1)
+//     20 x 400 x 600 x 8                                      96 (4)      41 (1)      35 (1)
+//     40 x 569 x 416 x 4                                      79 (5)      62 (1)
+struct ScanForm {
+    int lanes, per_lane;
+    double ns, alone, start;
+};
+constexpr ScanForm kForms[] = {{4, 1, 71, 1.15, 0}, {8, 1, 31, 1.7, 0}, {1, 16, 285, 1.8, 2}, {8, 2, 49, 1.45, 0}, {16, 1, 31, 1.5, 0}, {8, 4, 75, 1.5, 0}, {16, 2, 45, 1.25, 0}, {16, 4, 96, 1.1, 0}};
+
+// Few channels leave SIMDs empty: then fewer states for each lane, or pieces along the positions, which cost a pass for their ends (0.6 of the
+// main one) and a launch that joins them (8 us).  The choice is the cheapest by these numbers and the waves that a SIMD (1024 of them) runs.
 static bool plan_scan(const tae_scan_args* p, ScanPlan* out) {
     if (p->batch < 1 || p->len < 1 || p->channels < 1 || p->states < 1 || p->states > 64 || !dtype_ok(p->dtype)) return false;
     if (p->len == 1) return true;
     int padded = 4;
     while (padded < p->states) padded *= 2;
     double least = 0.0;
-    for (int form = 0; form < 7; ++form) {
-        const int tiled = form >= 3, lanes = tiled ? 2 << (form - 3) : 1 << form, per_lane = padded / lanes;
-        if (lanes > padded || (tiled ? per_lane > 4 : per_lane < 4 || per_lane > 32)) continue;
-        const int64_t groups = ceil_div(p->channels, tiled ? kScanThreads / lanes : 64 / lanes), waves = tiled ? 4 : 1;
-        const double channel = tiled ? 1.0 / lanes : 1.0, across = tiled ? 18.0 : lanes > 1 ? 4.0 : 0.0;
+    for (const ScanForm& f : kForms) {
+        if (f.lanes * f.per_lane != padded) continue;
+        const int64_t groups = ceil_div(p->channels, f.lanes == 1 ? 64 : kScanThreads / f.lanes), waves = f.lanes == 1 ? 1 : 4;
         for (int64_t pieces = 1; pieces <= 64; ++pieces) {
             const int64_t piece_len = ceil_div(ceil_div(p->len, pieces), kPieceUnit) * kPieceUnit;
             if (ceil_div(p->len, piece_len) < pieces) continue;
-            // waves of a SIMD, three at a time at the most; a wave starts with about 3 us of loads
-            auto time = [&](int64_t n, double ns) {
-                const double all = std::ceil(n * waves * p->batch * groups / 1024.0 * 4.0) / 4.0, whole = std::floor(all / 3.0), rest = all - 3.0 * whole;
-                return (3.0 * whole + (rest > 0.0 ? std::max(2.0, rest) : 0.0)) * std::min<int64_t>(piece_len, p->len) * ns + (whole + (rest > 0.0)) * 3000.0;
+            auto time = [&](int64_t n) {
+                const double all = std::ceil(n * waves * p->batch * groups / 1024.0 * 4.0) / 4.0;
+                return std::max(all, f.alone) * std::min<int64_t>(piece_len, p->len) * f.ns * 1e-3 + f.start * std::max(all, 1.0);
             };
-            double cost = time(pieces, 12.4 * per_lane + 55.0 * channel + across);
-            if (pieces > 1) cost += time(pieces - 1, 10.4 * per_lane + 30.0 * channel + across) + 9000.0;
+            const double cost = time(pieces) + (pieces > 1 ? 0.6 * time(pieces - 1) + 8.0 : 0.0);
             if (least == 0.0 || cost < least) {
                 least = cost;
-                out->lanes = lanes;
-                out->per_lane = per_lane;
-                out->tiled = tiled;
+                out->lanes = f.lanes;
+                out->per_lane = f.per_lane;
                 out->groups = (int)groups;
                 out->pieces = (int)pieces;
                 out->piece_len = (int)piece_len;
@@ -709,43 +714,29 @@ static int launch_scan(const ScanArgs& a, bool vector, int64_t batch, hipStream_
     return TAE_OK;
 }
 
-template <class T, int N, int P>
+template <class T, int N>
 static int launch_lane(const ScanArgs& a, int64_t batch, hipStream_t st) {
     const dim3 grid = grid_of(ceil_div(a.blocks, kLaneWaves)), block(kLaneWaves * 64);
     if (a.pieces > 1) {
-        hipLaunchKernelGGL((scan_lane_kernel<T, N, P, true>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((scan_lane_kernel<T, N, true>), grid, block, 0, st, a);
         launch_join(a, batch, st);
     }
-    hipLaunchKernelGGL((scan_lane_kernel<T, N, P, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((scan_lane_kernel<T, N, false>), grid, block, 0, st, a);
     return TAE_OK;
 }
 
 template <class T>
 static int launch_scan_plan(const ScanArgs& a, const ScanPlan& s, bool v, int batch, hipStream_t st) {
     if (a.len == 1) return v ? launch_steps<T, 4>(a, batch, st) : launch_steps<T, 1>(a, batch, st);
-    switch (s.tiled * 10000 + s.lanes * 100 + s.per_lane) {
-        case 104: return launch_lane<T, 4, 1>(a, batch, st);
-        case 108: return launch_lane<T, 8, 1>(a, batch, st);
-        case 116: return launch_lane<T, 16, 1>(a, batch, st);
-        case 132: return launch_lane<T, 32, 1>(a, batch, st);
-        case 204: return launch_lane<T, 4, 2>(a, batch, st);
-        case 208: return launch_lane<T, 8, 2>(a, batch, st);
-        case 216: return launch_lane<T, 16, 2>(a, batch, st);
-        case 232: return launch_lane<T, 32, 2>(a, batch, st);
-        case 404: return launch_lane<T, 4, 4>(a, batch, st);
-        case 408: return launch_lane<T, 8, 4>(a, batch, st);
-        case 416: return launch_lane<T, 16, 4>(a, batch, st);
-        case 10202: return launch_scan<T, 2, 2, 16>(a, v, batch, st);
-        case 10204: return launch_scan<T, 4, 2, 16>(a, v, batch, st);
-        case 10401: return launch_scan<T, 1, 4, 32>(a, v, batch, st);
-        case 10402: return launch_scan<T, 2, 4, 32>(a, v, batch, st);
-        case 10404: return launch_scan<T, 4, 4, 32>(a, v, batch, st);
-        case 10801: return launch_scan<T, 1, 8, 32>(a, v, batch, st);
-        case 10802: return launch_scan<T, 2, 8, 32>(a, v, batch, st);
-        case 10804: return launch_scan<T, 4, 8, 32>(a, v, batch, st);
-        case 11601: return launch_scan<T, 1, 16, 64>(a, v, batch, st);
-        case 11602: return launch_scan<T, 2, 16, 64>(a, v, batch, st);
-        case 11604: return launch_scan<T, 4, 16, 64>(a, v, batch, st);
+    switch (s.lanes * 100 + s.per_lane) {
+        case 116: return launch_lane<T, 16>(a, batch, st);
+        case 401: return launch_scan<T, 1, 4, 32>(a, v, batch, st);
+        case 801: return launch_scan<T, 1, 8, 32>(a, v, batch, st);
+        case 802: return launch_scan<T, 2, 8, 32>(a, v, batch, st);
+        case 804: return launch_scan<T, 4, 8, 32>(a, v, batch, st);
+        case 1601: return launch_scan<T, 1, 16, 64>(a, v, batch, st);
+        case 1602: return launch_scan<T, 2, 16, 64>(a, v, batch, st);
+        case 1604: return launch_scan<T, 4, 16, 64>(a, v, batch, st);
     }
     return fail_msg(TAE_EINVAL, "internal: selective_scan has no kernel for this plan");
 }
