@@ -64,9 +64,18 @@ struct Raw {
             }
         }
     }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = 0;
+    // from an address that is aligned to its elements only
+    __device__ __forceinline__ void from_any(const T* p) { __builtin_memcpy(w, p, BYTES); }
+    // without its first n elements (0 to 3), those behind them moved up, zeros at the end: 4 elements
+    __device__ __forceinline__ void drop(int n) {
+        static_assert(V == 4, "four elements");
+        if constexpr (sizeof(T) == 2) {
+            const uint64_t u = ((uint64_t)w[1] << 32 | w[0]) >> (16 * n);
+            w[0] = (uint32_t)u, w[1] = (uint32_t)(u >> 32);
+        } else {
+            if (n & 1) w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = 0;
+            if (n & 2) w[0] = w[2], w[1] = w[3], w[2] = w[3] = 0;
+        }
     }
     __device__ __forceinline__ float operator[](int i) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);

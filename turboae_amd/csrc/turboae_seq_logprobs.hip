@@ -157,7 +157,12 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
             if (at < low || at > high) {
                 Pack<T, V> p;
 #pragma unroll
-                for (int i = 0; i < V; ++i) p.v[i] = at + i >= lo && at + i < hi ? x[at + i] : (T)kNegInf;
+                for (int i = 0; i < V; ++i) p.v[i] = (T)kNegInf;
+                if (at + V > lo && at < hi) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (at + i >= lo && at + i < hi) p.v[i] = x[at + i];
+                }
                 const uint4 u = __builtin_bit_cast(uint4, p);
                 w[g][0] = u.x, w[g][1] = u.y, w[g][2] = u.z, w[g][3] = u.w;
             }
@@ -315,16 +320,24 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
         }
     }
     // the largest key of this lane's elements that is below `limit`
-    auto best_below = [&](u64 limit) {           // read again, so that this rare way costs the usual one no registers
+    auto best_below = [&](u64 limit) {
         u64 best = 0;
-#pragma unroll 1
-        for (int g = 0; g < G; ++g)
-#pragma unroll 1
-            for (int i = 0; i < V; ++i) {
-                const int at = place(g) + i;
-                const u64 k = at >= lo && at < hi ? key_of((float)x[at], at) : 0;
+        if constexpr (W < 64) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const u64 k = place(g) < hi ? key_of(value(g, 0), place(g)) : 0;
                 best = k > best && k < limit ? k : best;
             }
+        } else {                                 // read again, so that this rare way costs the usual one no registers
+#pragma unroll 1
+            for (int g = 0; g < G; ++g)
+#pragma unroll 1
+                for (int i = 0; i < V; ++i) {
+                    const int at = place(g) + i;
+                    const u64 k = at >= lo && at < hi ? key_of((float)x[at], at) : 0;
+                    best = k > best && k < limit ? k : best;
+                }
+        }
         return best;
     };
     u64 best = best_below(~0ull);
@@ -421,7 +434,7 @@ static bool plan_logprobs(const tae_logprobs_args* p, bool aligned_rows, Logprob
     // the fewest lanes that hold a row; long rows in parts, smaller ones where few rows would leave SIMDs empty
     const int64_t elements = (int64_t)p->rows * p->vocab;
     if (p->vocab <= 64) parts_of(8, 8);
-    else if (p->vocab <= 512 - spare) parts_of(64, 8);
+    else if (p->vocab <= 512 - spare) parts_of(64, 8);      // single elements: all lanes have some, and so a close bound of the alternatives
     else if (p->vocab <= 2048 - spare || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32);
     else if (p->vocab <= 8192 - spare || (elements < (int64_t)1024 * 8192 && p->vocab <= (1 << 20))) parts_of(256, 32);
     else parts_of(256, 64);
@@ -437,7 +450,7 @@ static void launch_logprobs(const LogprobsArgs& a, const LogprobsPlan& s, hipStr
     constexpr int V = 16 / sizeof(T);
     const int64_t units = (int64_t)a.rows * a.parts;
     if (s.lanes == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 8, 8, 1, 256>), grid_of(ceil_div(units, 32)), dim3(256), 0, st, a);
-    else if (s.lanes == 64 && s.ept == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, V, 64>), grid_of(units), dim3(64), 0, st, a);
+    else if (s.lanes == 64 && s.ept == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, 1, 64>), grid_of(units), dim3(64), 0, st, a);
     else if (s.lanes == 64) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 32, V, 64>), grid_of(units), dim3(64), 0, st, a);
     else if (s.ept == 32) hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 32, V, 256>), grid_of(units), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 64, V, 256>), grid_of(units), dim3(256), 0, st, a);

@@ -49,7 +49,7 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
     return v;
 }
 
-template <class T, class R, int V, int NV, int TPR, int THREADS>
+template <class T, class R, int V, int NV, int TPR, int THREADS, bool EDGE>
 __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
     __shared__ float lds[16];
     const int lane = threadIdx.x % TPR;
@@ -67,16 +67,44 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
     constexpr bool GATE_AHEAD = NV * V < 32;
     Raw<R, V> raw_r[NV];
     Raw<T, V> raw_p[NV], raw_g[GATE_AHEAD ? NV : 1];
+    const int over = EDGE ? (a.dim + V - 1) / V * V - a.dim : 0;            // by how much the last V reach past the row
+    auto fetch = [&](auto& raw, const auto* from, int e) {
+        if constexpr (EDGE) raw.from_any(from + min(e, a.dim - V));
+        else raw.from(from + min(e, a.dim - V));
+    };
+    auto settle = [&](auto& raw, int e) {       // EDGE: the last V of a row were loaded `over` elements early
+        if constexpr (EDGE) raw.drop(e < a.dim && e + V > a.dim ? over : 0);
+    };
+    auto place = [&](int j) { return (j * TPR + lane) * V; };
 #pragma unroll
-    for (int j = 0; j < NV; ++j) raw_r[j].from(rs + min((j * TPR + lane) * V, a.dim - V));
+    for (int j = 0; j < NV; ++j) fetch(raw_r[j], rs, place(j));
     if (a.block) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) raw_p[j].from(bl + min((j * TPR + lane) * V, a.dim - V));
+        for (int j = 0; j < NV; ++j) fetch(raw_p[j], bl, place(j));
         if (GATE_AHEAD && a.gate) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) raw_g[GATE_AHEAD ? j : 0].from(ga + min((j * TPR + lane) * V, a.dim - V));
+            for (int j = 0; j < NV; ++j) fetch(raw_g[GATE_AHEAD ? j : 0], ga, place(j));
         }
     }
+    auto vector = [&](const float* from, int e) {
+        Raw<float, V> w;
+        fetch(w, from, e);
+        settle(w, e);
+        return w;
+    };
+    auto put = [&](auto* to, const auto& x, int e) {
+        if constexpr (EDGE) {
+            if (e + V <= a.dim) {
+                store_any(to + e, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (e + i < a.dim) to[e + i] = x.v[i];
+            }
+        } else {
+            store(to + e, x);
+        }
+    };
     float r[NV][V];
     auto norm_of = [&](const float (&v)[NV][V], float& mean, float& rstd) {
         mean = 0.0f;
@@ -91,10 +119,10 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const bool in = (j * TPR + lane) * V < a.dim;
+            const int e = place(j);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = in ? v[j][i] - mean : 0.0f;
+                const float d = e + (EDGE ? i : 0) < a.dim ? v[j][i] - mean : 0.0f;
                 s = __builtin_fmaf(d, d, s);
             }
         }
@@ -102,9 +130,11 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
     };
     auto unpack = [&](float (&v)[NV][V], auto& raw) {        // zeros behind the row
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            settle(raw[j], place(j));
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[j][i] = (j * TPR + lane) * V < a.dim ? raw[j][i] : 0.0f;
+            for (int i = 0; i < V; ++i) v[j][i] = place(j) < a.dim ? raw[j][i] : 0.0f;
+        }
     };
     if (a.block) {
         float p[NV][V];
@@ -113,29 +143,30 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
         if (a.post_w) norm_of(p, mean, rstd);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = (j * TPR + lane) * V;
+            const int e = place(j);
             if (e >= a.dim) continue;
             float f[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) f[i] = p[j][i];
             if (a.post_w) {
-                const Pack<float, V> w = load<float, V>(a.post_w + e);
+                const Raw<float, V> w = vector(a.post_w, e);
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] = (f[i] - mean) * rstd * w.v[i];
+                for (int i = 0; i < V; ++i) f[i] = (f[i] - mean) * rstd * w[i];
                 if (a.post_b) {
-                    const Pack<float, V> c = load<float, V>(a.post_b + e);
+                    const Raw<float, V> c = vector(a.post_b, e);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) f[i] += c.v[i];
+                    for (int i = 0; i < V; ++i) f[i] += c[i];
                 }
             }
             if (a.scale) {
-                const Pack<float, V> w = load<float, V>(a.scale + e);
+                const Raw<float, V> w = vector(a.scale, e);
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] *= w.v[i];
+                for (int i = 0; i < V; ++i) f[i] *= w[i];
             }
             if (a.gate) {
                 Raw<T, V>& g = raw_g[GATE_AHEAD ? j : 0];
-                if (!GATE_AHEAD) g.from(ga + e);
+                if (!GATE_AHEAD) fetch(g, ga, e);
+                settle(g, e);
 #pragma unroll
                 for (int i = 0; i < V; ++i) f[i] *= gate_value(g[i], a.gate_act);
             }
@@ -154,12 +185,12 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
         R* o = (R*)a.out + b * a.ou_b + t * a.ou_r;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = (j * TPR + lane) * V;
+            const int e = place(j);
             if (e >= a.dim) continue;
             Pack<R, V> x;
 #pragma unroll
             for (int i = 0; i < V; ++i) x.v[i] = (R)r[j][i];
-            store<R, V>(o + e, x);
+            put(o, x, e);
         }
     }
     if (a.normed) {
@@ -168,52 +199,52 @@ __global__ __launch_bounds__(THREADS) void norm_residual_kernel(NormArgs a) {
         T* o = (T*)a.normed + row * a.dim;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = (j * TPR + lane) * V;
+            const int e = place(j);
             if (e >= a.dim) continue;
-            const Pack<float, V> w = load<float, V>(a.pre_w + e);
+            const Raw<float, V> w = vector(a.pre_w, e);
             float f[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = (r[j][i] - mean) * rstd * w.v[i];
+            for (int i = 0; i < V; ++i) f[i] = (r[j][i] - mean) * rstd * w[i];
             if (a.pre_b) {
-                const Pack<float, V> c = load<float, V>(a.pre_b + e);
+                const Raw<float, V> c = vector(a.pre_b, e);
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] += c.v[i];
+                for (int i = 0; i < V; ++i) f[i] += c[i];
             }
             Pack<T, V> x;
 #pragma unroll
             for (int i = 0; i < V; ++i) x.v[i] = (T)f[i];
-            store<T, V>(o + e, x);
+            put(o, x, e);
         }
     }
 }
 
-template <class T, class R, int V, int NV, int TPR, int THREADS>
+template <class T, class R, int V, int NV, int TPR, int THREADS, bool EDGE>
 static void launch_norm_as(const NormArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((norm_residual_kernel<T, R, V, NV, TPR, THREADS>), grid_of(ceil_div(a.rows, THREADS / TPR)), dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((norm_residual_kernel<T, R, V, NV, TPR, THREADS, EDGE>), grid_of(ceil_div(a.rows, THREADS / TPR)), dim3(THREADS), 0, st, a);
 }
 
 // Lanes and steps of V that hold a row: part of a wave for short rows, then a wave, then a workgroup.
-template <class T, class R, int V>
+template <class T, class R, int V, bool EDGE>
 static void launch_norm_width(const NormArgs& a, hipStream_t st) {
     const int vecs = (int)ceil_div(a.dim, V);
-    constexpr int M = V == 1 ? 4 : 1;           // single elements: four for each lane at least
-    if (vecs <= 16 * M) launch_norm_as<T, R, V, M, 16, 256>(a, st);
-    else if (vecs <= 32 * M) launch_norm_as<T, R, V, M, 32, 256>(a, st);
-    else if (vecs <= 64 * M) launch_norm_as<T, R, V, M, 64, 256>(a, st);
-    else if (vecs <= 128 * M) launch_norm_as<T, R, V, 2 * M, 64, 256>(a, st);
-    else if (vecs <= 256 * M) launch_norm_as<T, R, V, M, 256, 256>(a, st);
-    else if (vecs <= 512 * M) launch_norm_as<T, R, V, 2 * M, 256, 256>(a, st);
-    else if (vecs <= 1024 * M) launch_norm_as<T, R, V, 4 * M, 256, 256>(a, st);
-    else if (vecs <= 2048 * M) launch_norm_as<T, R, V, 2 * M, 1024, 1024>(a, st);
-    else if (V == 8 || vecs <= 4096 * M) launch_norm_as<T, R, V, 4 * M, 1024, 1024>(a, st);
-    else if constexpr (V < 8) launch_norm_as<T, R, V, 8 * M, 1024, 1024>(a, st);
+    if (vecs <= 16) launch_norm_as<T, R, V, 1, 16, 256, EDGE>(a, st);
+    else if (vecs <= 32) launch_norm_as<T, R, V, 1, 32, 256, EDGE>(a, st);
+    else if (vecs <= 64) launch_norm_as<T, R, V, 1, 64, 256, EDGE>(a, st);
+    else if (vecs <= 128) launch_norm_as<T, R, V, 2, 64, 256, EDGE>(a, st);
+    else if (vecs <= 256) launch_norm_as<T, R, V, 1, 256, 256, EDGE>(a, st);
+    else if (vecs <= 512) launch_norm_as<T, R, V, 2, 256, 256, EDGE>(a, st);
+    else if (vecs <= 1024) launch_norm_as<T, R, V, 4, 256, 256, EDGE>(a, st);
+    else if (vecs <= 2048) launch_norm_as<T, R, V, 2, 1024, 1024, EDGE>(a, st);
+    else if (V == 8 || vecs <= 4096) launch_norm_as<T, R, V, 4, 1024, 1024, EDGE>(a, st);
+    else if constexpr (V < 8) launch_norm_as<T, R, V, 8, 1024, 1024, EDGE>(a, st);
 }
 
 template <class T, class R>
 static void launch_norm(const NormArgs& a, int width, hipStream_t st) {
-    if (width == 8) launch_norm_width<T, R, 8>(a, st);
-    else if (width == 4) launch_norm_width<T, R, 4>(a, st);
-    else launch_norm_width<T, R, 1>(a, st);
+    if (width == 8) launch_norm_width<T, R, 8, false>(a, st);
+    else if (width == 4) launch_norm_width<T, R, 4, false>(a, st);
+    else if (a.dim >= 4) launch_norm_width<T, R, 4, true>(a, st);
+    else launch_norm_as<T, R, 1, 1, 16, 256, false>(a, st);
 }
 
 }  // namespace seq
