@@ -42,7 +42,8 @@ __device__ __forceinline__ Pack<int8_t, V> whole_numbers(const Pack<T, V>& p, fl
 }
 
 // One workgroup for each row, which stays in registers (KEEP groups of V for each lane; a row holds one at least) or, with KEEP = 0, is read
-// twice.  Rows may start on any element: wide loads need no more here.
+// twice.  Rows may start on any element: wide loads need no more here.  Bound by memory and by issuing at once: 8192 x 4096 in bf16 (101 MB)
+// 22 us, 4.5 TB/s, vector instructions 95 % of the time; 4 x 4096 3.2 us, most of it starting up.
 template <class T, int V, int KEEP>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     __shared__ float lds[4];
@@ -195,6 +196,11 @@ __device__ __forceinline__ void wait_copies() {             // all but the last 
 // under way.  A row's eight 16-byte pieces are permuted by its number (by which piece a lane copies), so that the 16 lanes which read LDS
 // together touch all banks.  Weight rows are dealt to fragments such that a lane ends up with 16 adjacent outputs.  Workgroups of one XCD
 // (every eighth) take adjacent tiles, eight rows of tiles high, and share operands in its L2.
+//
+// Measured, bf16, 8192 x 4096 x 8192 (550 G operations): 230 us among other work and 263 to 285 in a row, by the power that is left: 1.9 to 2.4 POP/s.
+// A stream of nothing but these matrix instructions on such numbers reaches 3.7, a large library product 1.8.  The matrix pipes are busy half
+// of the cycles; the rest are waits for fragments and copies at 61 bytes a clock for each CU.  Slower: a ring of five buffers of 64 inputs
+// (requests of half a line), waves of 128 x 128 (spills), 128 x 128 tiles (4096 x 4096 x 4096: 91 us, these 83).
 template <class T, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64, BM / WM * (BN / WN) > 8192 ? 1 : 2) void int8_linear_kernel(Int8Args a) {
     constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, ROWS = BM + BN, PIECES = ROWS / 8 / WAVES, STAGE = ROWS * 128;
@@ -353,6 +359,7 @@ __global__ __launch_bounds__(WM * WN * 64, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
 
 // Few rows of x: bound by reading the weights.  16 NF weight rows and up to 16 MF rows of x for each workgroup; its eight waves share the
 // inputs and join their sums, exact in any order, in LDS.  Both operands come straight from memory (x from L2), DEEP slabs of 64 in flight.
+// Measured: 4 x 4096 x 4096 6.1 us, 2.8 TB/s of weights with start and drain.
 template <class T, int MF, int NF, int DEEP>
 __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
     constexpr int FRAGMENTS = MF * NF, ROUND = FRAGMENTS < 8 ? FRAGMENTS : 8;          // joined at once

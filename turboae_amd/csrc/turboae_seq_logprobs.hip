@@ -1,8 +1,12 @@
 // tae_token_logprobs: log probability of a given token, entropy and the most probable tokens of each row of logits.
 //
 // Bound by memory.  A row, or a part of a long one, is read once into registers; its maximum m, s = sum e^(x - m) and t = sum (x - m) e^(x - m)
-// give log p = x - m - log s and the entropy log s - t / s, and parts join by rescaling to the largest m.  Alternatives are picked one by
-// one: elements are ordered by a 64-bit key (value, then the lower index), all different, so that every choice of parts gives the same ids.
+// give log p = x - m - log s and the entropy log s - t / s, and parts join by rescaling to the largest m.  Elements are ordered by a 64-bit
+// key (value, then the lower index), all different, so that every choice of parts gives the same ids.
+//
+// Measured, bf16, 2048 x 131072 with 8 alternatives (537 MB): 106 to 124 us, 4.3 to 5.1 TB/s (a large copy: 5.2), 8 of them the join.  14.5
+// vector instructions for each element of a lane keep the SIMDs as busy as memory: taking each of bf16's elements apart once and holding it
+// costs more (157 us: half the waves), parts of 512 lanes more too.  8 x 50001 in fp32 with 20: 7 us and 5 for the join, mostly waiting.
 #include "turboae_seq.hpp"
 
 namespace tae {
