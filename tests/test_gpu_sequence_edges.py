@@ -165,3 +165,25 @@ def test_infinite_inputs_stay_in_their_channel(gpu_device):
     other[1, 100:, 5] = False
     assert torch.equal(y.cpu()[other], clean[0].cpu()[other])
     assert not bool(torch.isfinite(y[1, 100, 5])) and not bool(torch.isfinite(h[1, 5]).any())
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("K", [1, 15, 64, 100, 511, 1000, 3001, 9000])
+def test_int8_of_few_rows(gpu_device, dt, K):
+    """1 to 17 rows, with one of zeros, one with a NaN and one with an infinity, which spoil only themselves; rows on any element."""
+    from turboae_amd import sequence
+    dev, t = gpu_device, DT[dt]
+    for M in (1, 2, 3, 4, 5, 8, 9, 16, 17):
+        for N in (1, 17, 40):
+            g = gen(M * 1000 + K + N)
+            x, w = rnd(g, M, K, dtype=t), torch.randint(-127, 128, (N, -(-K // 16) * 16), generator=g, dtype=torch.int8)
+            s, b = torch.rand(N, generator=g), rnd(g, N)
+            if M > 4:
+                x[1], x[2, K // 2], x[4, K - 1] = 0.0, NAN, -INF
+            keep = [i for i in range(M) if M <= 4 or i not in (2, 4)]
+            y, bound = O.int8_linear(x[keep], w[:, :K], s, b)
+            buf = torch.full((M, K + 3), NAN, dtype=t, device=dev)
+            buf[:, 1:K + 1] = x.to(dev)
+            got = sequence.int8_linear(buf[:, 1:K + 1], w.to(dev)[:, :K], s.to(dev), b.to(dev))
+            inside(got[keep], y, bound, (M, N))
+            assert len(keep) == M or bool(torch.isnan(got[[2, 4]]).all())

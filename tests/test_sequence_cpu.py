@@ -47,7 +47,7 @@ def norm():
 
 
 def int8():
-    return build(_lib.TaeInt8Args, rows=2, inputs=32, outputs=4, x_row=32, weight_row=32, x=PTR, weight=PTR, weight_scale=PTR, y=PTR)
+    return build(_lib.TaeInt8Args, rows=40, inputs=32, outputs=4, x_row=32, weight_row=32, x=PTR, weight=PTR, weight_scale=PTR, y=PTR)
 
 
 def logprobs():
@@ -98,7 +98,9 @@ def test_quantize_refuses():
 def test_workspaces_are_sized_without_tensors():
     lib = _lib.load()
     a = int8()
-    assert lib.tae_int8_linear_workspace(C.byref(a)) >= 2 * 32 + 8
+    assert lib.tae_int8_linear_workspace(C.byref(a)) >= 40 * 32 + 160
+    a.rows = 2
+    assert lib.tae_int8_linear_workspace(C.byref(a)) == 0                        # few rows are quantised where they are used
     assert lib.tae_int8_linear_workspace(C.byref(build(_lib.TaeInt8Args, rows=0, inputs=4, outputs=4))) == 0
     assert lib.tae_selective_scan_workspace(C.byref(scan())) > 0
     one = scan()

@@ -41,9 +41,32 @@ __device__ __forceinline__ Pack<int8_t, V> whole_numbers(const Pack<T, V>& p, fl
     return o;
 }
 
+// The largest magnitude by its bits, which are ordered as the magnitudes are, two 16-bit ones at once; an infinity or NaN is infinite.
+template <class T>
+struct Largest {
+    using Halves = __attribute__((ext_vector_type(2))) uint16_t;
+    uint32_t bits = 0;
+    template <int V>
+    __device__ __forceinline__ void look(const Pack<T, V>& p) {
+        uint32_t w[sizeof(p) / 4];
+        __builtin_memcpy(w, &p, sizeof(p));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(p) / 4; ++i) {
+            if constexpr (sizeof(T) == 4) bits = max(bits, w[i] & 0x7FFFFFFFu);
+            else bits = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(Halves, bits), __builtin_bit_cast(Halves, w[i] & 0x7FFF7FFFu)));
+        }
+    }
+    __device__ __forceinline__ float value() const {
+        float v;
+        if constexpr (sizeof(T) == 4) v = __uint_as_float(bits);
+        else v = (float)__builtin_bit_cast(T, (uint16_t)max(bits & 0xFFFFu, bits >> 16));
+        return v < __builtin_inff() ? v : __builtin_inff();
+    }
+};
+
 // One workgroup for each row, which stays in registers (KEEP groups of V for each lane; a row holds one at least) or, with KEEP = 0, is read
 // twice.  Rows may start on any element: wide loads need no more here.  Bound by memory and by issuing at once: 8192 x 4096 in bf16 (101 MB)
-// 22 us, 4.5 TB/s, vector instructions 95 % of the time; 4 x 4096 3.2 us, most of it starting up.
+// 22 us, 4.5 TB/s, vector instructions 95 % of the time when magnitudes were compared as floats, by bits 21; 4 x 4096 3.2 us, most of it starting up.
 template <class T, int V, int KEEP>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     __shared__ float lds[4];
@@ -51,16 +74,7 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
     if (row >= a.rows) return;
     const int tid = threadIdx.x;
     const T* x = (const T*)a.x + row * a.x_r;
-    float most = 0.0f;
-    bool bad = false;
-    auto look = [&](const Pack<T, V>& p) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float v = fabsf((float)p.v[i]);
-            bad = bad || !(v < __builtin_inff());
-            most = fmaxf(most, v);
-        }
-    };
+    Largest<T> largest;
     auto edge = [&](int e) {                     // the last group of a row, zeros behind it
         Pack<T, V> p;
 #pragma unroll
@@ -75,15 +89,14 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(QuantArgs a) {
         for (int j = 0; j < KEEP; ++j) {
             const int e = (j * 256 + tid) * V;
             if (e < a.cols && e + V > a.cols) kept[j] = edge(e);
-            look(kept[j]);
+            largest.look(kept[j]);
         }
     } else {
         int e = tid * V;
-        for (; e + V <= a.cols; e += 256 * V) look(load_any<T, V>(x + e));
-        if (e < a.cols) look(edge(e));
+        for (; e + V <= a.cols; e += 256 * V) largest.look(load_any<T, V>(x + e));
+        if (e < a.cols) largest.look(edge(e));
     }
-    if (__any(bad)) most = __builtin_inff();
-    most = lanes_max<64>(most);
+    float most = lanes_max<64>(largest.value());
     if ((tid & 63) == 0) lds[tid >> 6] = most;
     __syncthreads();
     most = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
@@ -421,6 +434,91 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
     }
 }
 
+// Up to 8 rows of x in one launch: every workgroup quantises all of them itself, into LDS, with its first weights under way, and goes on like
+// int8_few_kernel with 16 weight rows.  `share` waves share a row.  Measured in bf16 in a graph, then eagerly, against two launches: 4 x 1024 x
+// 1024 5.8 and 9.8 us (7.5 and 13.9), 1 x 4096 x 4096 7.7 and 9.7 (9.0 and 14.4), 4 x 4096 x 4096 9.3 and 9.8 (9.6 and 14.6).  More rows or
+// inputs take longer to quantise again and again than a launch (with 8 groups a lane, 8 x 4096 x 4096: 16.1 where two launches take 9.9), and
+// so do more workgroups than the CUs hold at once (1 x 1024 x 51200: 33 where two take 16).
+constexpr int kRowsGroups = 4;                   // groups of 16 bytes that a lane holds
+template <class T>
+__global__ __launch_bounds__(512) void int8_rows_kernel(Int8Args a, const T* x, int64_t x_r, int share) {
+    constexpr int V = 16 / sizeof(T), DEEP = 8;
+    __shared__ i32x4 part[8][64];
+    __shared__ float most_of[8], scale_of[8];
+    extern __shared__ char lds[];                // (m, q_r) whole numbers, zero behind k
+    const int64_t id = block_index();
+    if (id >= a.blocks) return;
+    const int n0 = (int)id * 16, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kk = (lane >> 4) * 16;
+    const int slabs = (a.k + 63) / 64, each = (slabs + 7) / 8, begin = wave * each, end = min(begin + each, slabs), last = (a.k - 1) & ~15;
+    const int8_t* w = a.w + (int64_t)min(n0 + r16, a.n - 1) * a.w_r;
+    i32x4 wv[DEEP];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) wv[d] = *(const i32x4*)(w + min(min(s0 + d, slabs - 1) * 64 + kk, last));
+    };
+    fetch(begin);
+    const int step = 64 * V * share, from = (wave % share * 64 + lane) * V, m = wave / share;
+    const T* row = x + m * x_r;
+    Pack<T, V> kept[kRowsGroups];
+    Largest<T> largest;
+    if (m < a.m) {
+        if (a.k >= V) {
+#pragma unroll
+            for (int i = 0; i < kRowsGroups; ++i) kept[i] = load_any<T, V>(row + min(from + i * step, a.k - V));
+        }
+#pragma unroll
+        for (int i = 0; i < kRowsGroups; ++i) {
+            const int e = from + i * step;
+            if (a.k < V || (e < a.k && e + V > a.k)) {            // the last group of the row, zeros behind it
+#pragma unroll
+                for (int c = 0; c < V; ++c) kept[i].v[c] = e + c < a.k ? row[e + c] : (T)0.0f;
+            }
+            largest.look(kept[i]);
+        }
+    }
+    float most = lanes_max<64>(largest.value());
+    if (lane == 0) most_of[wave] = most;
+    __syncthreads();
+    if (m < a.m) {
+        for (int i = 0; i < share; ++i) most = fmaxf(most, most_of[m * share + i]);
+        const bool fine = most < __builtin_inff();
+        if (lane == 0) scale_of[m] = fine ? most / 127.0f : __builtin_nanf("");
+        const float by = most > 0.0f ? most : 1.0f, reciprocal = 127.0f / by;
+        int8_t* q = (int8_t*)lds + m * (int)a.q_r;
+#pragma unroll
+        for (int i = 0; i < kRowsGroups; ++i) {
+            const int e = from + i * step;
+            if (e < slabs * 64) store<int8_t, V>(q + e, fine && e < a.k ? whole_numbers<T, V>(kept[i], by, reciprocal) : Pack<int8_t, V>{});
+        }
+    }
+    __syncthreads();
+    const char* q = lds + min(r16, a.m - 1) * (int)a.q_r + kk;
+    i32x4 acc = {};
+    for (int s0 = begin; s0 < end; s0 += DEEP) {
+        if (s0 > begin) fetch(s0);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (s0 + d < end) acc = mfma64(wv[d], *(const i32x4*)(q + (s0 + d) * 64), acc);
+    }
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+    i32x4 sum = part[0][lane];
+#pragma unroll
+    for (int u = 1; u < 8; ++u) sum += part[u][lane];
+    const int n = n0 + (lane >> 4) * 4;
+    if (r16 >= a.m || n >= a.n) return;
+    const Pack<T, 4> out = Outputs<T, 4>(a, n).row({sum[0], sum[1], sum[2], sum[3]}, scale_of[r16]);
+    T* y = (T*)a.y + (int64_t)r16 * a.n + n;
+    if (n + 4 <= a.n) {
+        store_any(y, out);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (n + c < a.n) y[c] = out.v[c];
+    }
+}
+
 template <class T, int BM, int BN, int WM, int WN, int STAGES>
 static hipError_t launch_tiles(Int8Args a, hipStream_t st) {
     constexpr int bytes = STAGES * (BM + BN) * 128;
@@ -474,6 +572,22 @@ static hipError_t launch_int8(const Int8Args& a, hipStream_t st) {
     return launch_tiles<T, 128, 128, 2, 2, 4>(a, st);
 }
 
+// Whether int8_rows_kernel takes a call: its rows fit the registers of a workgroup (and so LDS, 16 bytes off multiples of 64 so that the rows
+// meet all banks), and the workgroups that repeat the quantising are few.
+constexpr int64_t kRowsBlocks = 512;
+static int rows_share(const tae_int8_args* p) { return p->rows == 1 ? 8 : p->rows == 2 ? 4 : p->rows <= 4 ? 2 : 1; }
+static bool int8_in_one(const tae_int8_args* p) {
+    const int64_t across = 64 * 16 / (int64_t)dtype_bytes(p->dtype) * rows_share(p);
+    return p->rows <= 8 && p->inputs <= across * kRowsGroups && ceil_div(p->outputs, 16) <= kRowsBlocks;
+}
+
+template <class T>
+static void launch_rows(Int8Args a, const tae_int8_args* p, hipStream_t st) {
+    a.q_r = ceil_div(p->inputs, 64) * 64 + 16;
+    a.blocks = ceil_div(a.n, 16);
+    hipLaunchKernelGGL((int8_rows_kernel<T>), dim3((uint32_t)a.blocks), dim3(512), a.m * a.q_r, st, a, (const T*)p->x, p->x_row, rows_share(p));
+}
+
 // Rows 1024 bytes and multiples apart would send a slab's lines of all rows to few channels of L2.
 static int64_t q_stride(int32_t k) {
     const int64_t r = ceil_div(k, 128) * 128;
@@ -505,7 +619,7 @@ int tae_quantize_int8(int32_t dtype, const void* x, int64_t x_row, int32_t rows,
 
 size_t tae_int8_linear_workspace(const tae_int8_args* p) {
     using namespace tae::seq;
-    if (!p || p->struct_size != (int32_t)sizeof(tae_int8_args) || !int8_sizes(p)) return 0;
+    if (!p || p->struct_size != (int32_t)sizeof(tae_int8_args) || !int8_sizes(p) || !dtype_ok(p->dtype) || int8_in_one(p)) return 0;
     return (size_t)p->rows * q_stride(p->inputs) + (size_t)p->rows * 4;
 }
 
@@ -517,17 +631,25 @@ int tae_int8_linear(const tae_int8_args* p, void* stream) {
     if (!int8_sizes(p)) return fail_msg(TAE_EINVAL, "int8_linear: inputs must be in 1..131072, rows and outputs in 1..2^30");
     if (!p->x || !p->weight || !p->weight_scale || !p->y) return fail_msg(TAE_EINVAL, "int8_linear: x, weight, weight_scale and y must not be NULL");
     if (!aligned(p->weight, 16) || p->weight_row % 16 || p->weight_row < p->inputs || p->weight_row > (1 << 23)) return fail_msg(TAE_EINVAL, "int8_linear: weight rows start on 16-byte boundaries (quantize_int8 lays them so), at most 2^23 bytes apart");
-    const size_t need = tae_int8_linear_workspace(p);
-    if (!p->workspace || p->workspace_bytes < need || !aligned(p->workspace, 16)) return fail_msg(TAE_EINVAL, "int8_linear: the workspace is missing, misaligned or smaller than tae_int8_linear_workspace");
+    const size_t need = tae_int8_linear_workspace(p);         // 0: in one launch
+    if (need && (!p->workspace || p->workspace_bytes < need || !aligned(p->workspace, 16))) return fail_msg(TAE_EINVAL, "int8_linear: the workspace is missing, misaligned or smaller than tae_int8_linear_workspace");
     if (!elements_aligned(dtype_bytes(p->dtype), p->x, p->y) || !elements_aligned(4, p->weight_scale, p->bias)) return fail_msg(TAE_EINVAL, "int8_linear: a pointer is not aligned to its elements");
     const int64_t qr = q_stride(p->inputs);
     int8_t* q = (int8_t*)p->workspace;
-    float* scale = (float*)(q + (size_t)p->rows * qr);
+    float* scale = need ? (float*)(q + (size_t)p->rows * qr) : nullptr;
     Width wy(dtype_bytes(p->dtype));
     wy.elements(p->outputs).pointer(p->y);
     const Int8Args a{q, p->weight, scale, p->weight_scale, p->bias, p->y, qr, p->weight_row, p->rows, p->inputs, p->outputs, 0, wy.fits(16), 0, 0};
     return guarded([&] {
         hipStream_t st = (hipStream_t)stream;
+        if (!need) {
+            switch (p->dtype) {
+                case TAE_DTYPE_F32: launch_rows<float>(a, p, st); break;
+                case TAE_DTYPE_F16: launch_rows<f16>(a, p, st); break;
+                default: launch_rows<bf16>(a, p, st); break;
+            }
+            return (int)TAE_OK;
+        }
         launch_quantize_dtype(QuantArgs{p->x, q, scale, p->x_row, qr, p->rows, p->inputs}, p->dtype, st);
         hipError_t e;
         switch (p->dtype) {
