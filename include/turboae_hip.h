@@ -435,7 +435,7 @@ typedef struct tae_int8_args {
     void* workspace;
     size_t workspace_bytes;
 } tae_int8_args;
-TAE_API size_t tae_int8_linear_workspace(const tae_int8_args* args);
+TAE_API size_t tae_int8_linear_workspace(const tae_int8_args* args);         /* reads the sizes and the dtype only; 0: none, or bad sizes */
 TAE_API int tae_int8_linear(const tae_int8_args* args, void* stream);
 
 /* Reading a model's answers: for each row of logits the log probability of the given token, the entropy (nats) and the `top` most probable
@@ -457,7 +457,7 @@ typedef struct tae_logprobs_args {
     void* workspace;
     size_t workspace_bytes;
 } tae_logprobs_args;
-TAE_API size_t tae_token_logprobs_workspace(const tae_logprobs_args* args);
+TAE_API size_t tae_token_logprobs_workspace(const tae_logprobs_args* args);  /* the same */
 TAE_API int tae_token_logprobs(const tae_logprobs_args* args, void* stream);
 
 TAE_API const char* tae_last_error(void);
