@@ -41,6 +41,18 @@ __device__ __forceinline__ Pack<T, V> load_any(const T* p) {
 template <class T, int V>
 __device__ __forceinline__ void store_any(T* p, const Pack<T, V>& a) { __builtin_memcpy(p, &a, sizeof(a)); }
 
+// Four elements of T in `w` without the first n of them (0 to 3), those behind them moved up, zeros at the end
+template <class T>
+__device__ __forceinline__ void drop_first(uint32_t* w, int n) {
+    if constexpr (sizeof(T) == 2) {
+        const uint64_t u = ((uint64_t)w[1] << 32 | w[0]) >> (16 * n);
+        w[0] = (uint32_t)u, w[1] = (uint32_t)(u >> 32);
+    } else {
+        if (n & 1) w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = 0;
+        if (n & 2) w[0] = w[2], w[1] = w[3], w[2] = w[3] = 0;
+    }
+}
+
 // V adjacent elements as they were loaded, in whole registers: an element is taken out when it is used, so that a load stays in flight until
 // then and 16-bit elements need no registers of their own.
 template <class T, int V>
@@ -66,16 +78,9 @@ struct Raw {
     }
     // from an address that is aligned to its elements only
     __device__ __forceinline__ void from_any(const T* p) { __builtin_memcpy(w, p, BYTES); }
-    // without its first n elements (0 to 3), those behind them moved up, zeros at the end: 4 elements
     __device__ __forceinline__ void drop(int n) {
         static_assert(V == 4, "four elements");
-        if constexpr (sizeof(T) == 2) {
-            const uint64_t u = ((uint64_t)w[1] << 32 | w[0]) >> (16 * n);
-            w[0] = (uint32_t)u, w[1] = (uint32_t)(u >> 32);
-        } else {
-            if (n & 1) w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = 0;
-            if (n & 2) w[0] = w[2], w[1] = w[3], w[2] = w[3] = 0;
-        }
+        drop_first<T>(w, n);
     }
     __device__ __forceinline__ float operator[](int i) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);

@@ -438,7 +438,7 @@ static bool plan_logprobs(const tae_logprobs_args* p, bool aligned_rows, Logprob
     // the fewest lanes that hold a row; long rows in parts, smaller ones where few rows would leave SIMDs empty
     const int64_t elements = (int64_t)p->rows * p->vocab;
     if (p->vocab <= 64) parts_of(8, 8);
-    else if (p->vocab <= 512 - spare) parts_of(64, 8);      // single elements: all lanes have some, and so a close bound of the alternatives
+    else if (p->vocab <= 512 - spare) parts_of(64, 8);      // with alternatives single elements: all lanes have some, and so a close bound of them
     else if (p->vocab <= 2048 - spare || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32);
     else if (p->vocab <= 8192 - spare || (elements < (int64_t)1024 * 8192 && p->vocab <= (1 << 20))) parts_of(256, 32);
     else parts_of(256, 64);
@@ -454,7 +454,8 @@ static void launch_logprobs(const LogprobsArgs& a, const LogprobsPlan& s, hipStr
     constexpr int V = 16 / sizeof(T);
     const int64_t units = (int64_t)a.rows * a.parts;
     if (s.lanes == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 8, 8, 1, 256>), grid_of(ceil_div(units, 32)), dim3(256), 0, st, a);
-    else if (s.lanes == 64 && s.ept == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, 1, 64>), grid_of(units), dim3(64), 0, st, a);
+    else if (s.lanes == 64 && s.ept == 8 && a.top) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, 1, 64>), grid_of(units), dim3(64), 0, st, a);
+    else if (s.lanes == 64 && s.ept == 8) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 8, V, 64>), grid_of(units), dim3(64), 0, st, a);
     else if (s.lanes == 64) hipLaunchKernelGGL((logprobs_part_kernel<T, 64, 32, V, 64>), grid_of(units), dim3(64), 0, st, a);
     else if (s.ept == 32) hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 32, V, 256>), grid_of(units), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((logprobs_part_kernel<T, 256, 64, V, 256>), grid_of(units), dim3(256), 0, st, a);

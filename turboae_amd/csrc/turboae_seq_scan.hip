@@ -20,10 +20,11 @@ struct ScanArgs {
 constexpr int kScanThreads = 256;
 
 // Elements of a row as they were loaded, in whole registers and taken out only when they are used, so that a load stays in flight until
-// then.  V = 4: four adjacent ones, one load; V = 1: four, a load each; V = 0: one.  Elements behind the row repeat its last ones.
+// then.  V = 4: four adjacent ones, aligned to them; V = 1: four on any element, those of the row's end moved back inside it until `settle`;
+// V = 0: one, those behind the row repeat its last.
 template <class T, int V>
 struct Loaded {
-    uint32_t w[V == 4 ? sizeof(T) : V == 1 ? 4 : 1];
+    uint32_t w[V ? sizeof(T) : 1];
     __device__ __forceinline__ static uint32_t one(const T* p) {
         if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(p);
         else return *reinterpret_cast<const uint16_t*>(p);
@@ -36,17 +37,29 @@ struct Loaded {
             const uint2 u = *reinterpret_cast<const uint2*>(row + min(at, width - 4));
             w[0] = u.x, w[1] = u.y;
         } else if constexpr (V == 1) {
+            if (width >= 4) {
+                __builtin_memcpy(w, row + min(at, width - 4), 4 * sizeof(T));
+            } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = one(row + min(at + i, width - 1));
+                for (int i = 0; i < 4; ++i) w[i] = one(row + min(at + i, width - 1));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[i] = one(row + min(at + 2 * i, width - 1)) | one(row + min(at + 2 * i + 1, width - 1)) << 16;
+            }
         } else {
             w[0] = one(row + min(at, width - 1));
+        }
+    }
+    __device__ __forceinline__ void settle(int at, int width) {
+        if constexpr (V == 1) {
+            if (width >= 4) drop_first<T>(w, min(max(at + 4 - width, 0), 3));
         }
     }
     __device__ __forceinline__ float operator[](int i) const {
         if constexpr (sizeof(T) == 4) {
             return __uint_as_float(w[i]);
         } else {
-            const uint32_t u = V != 4 ? w[i] : i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
+            const uint32_t u = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
             return (float)__builtin_bit_cast(T, (uint16_t)u);
         }
     }
@@ -179,9 +192,12 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
         }
     };
     // positions at or behind `stop` get step 0: they keep the state.  What was repeated is replaced, not multiplied by 0: it may be infinite
-    auto stage = [&](const Raw& r, int t0, int buf) {
+    auto stage = [&](Raw& r, int t0, int buf) {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
+            r.x[j].settle(e0 + cq, E);
+            r.dt[j].settle(e0 + cq, E);
+            if constexpr (!ENDS) r.z[j].settle(e0 + cq, E);
             const int t = (j * kScanThreads + tid) / CQ;
             const bool in = t0 + t < stop;
 #pragma unroll
@@ -230,8 +246,7 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
                 b4[s] = load<float, 4>(&sb[buf][(s * P + p) * DS]);
                 if constexpr (!ENDS) c4[s] = load<float, 4>(&sc[buf][(s * P + p) * DS]);
             }
-#pragma unroll 4
-            for (int t = 0; t < TT; t += 4) {
+            auto four = [&](int t) {
                 // the next four positions' operands are read while these are worked on (at the last, four floats of padding)
                 const Pack<float, 4> dn = load<float, 4>(pd + t + 4), xn = load<float, 4>(px + t + 4);
                 Pack<float, 4> bn[S], cn[S];
@@ -280,6 +295,13 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
                     b4[s] = bn[s];
                     if constexpr (!ENDS) c4[s] = cn[s];
                 }
+            };
+            if (stop - t0 >= TT) {
+#pragma unroll 4
+                for (int t = 0; t < TT; t += 4) four(t);
+            } else {                             // no more than there are, rounded up: steps behind them are 0
+#pragma unroll 1
+                for (int t = 0; t < stop - t0; t += 4) four(t);
             }
         }
         if (more) stage(next, t0 + TT, buf ^ 1);
@@ -302,6 +324,8 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
                 T* to = y + (int64_t)at * E + e0 + cq;
                 if constexpr (V == 4) {
                     store<T, 4>(to, o);
+                } else if (e0 + cq + 4 <= E) {
+                    store_any(to, o);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
