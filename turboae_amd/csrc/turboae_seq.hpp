@@ -77,7 +77,10 @@ struct Raw {
         }
     }
     // from an address that is aligned to its elements only
-    __device__ __forceinline__ void from_any(const T* p) { __builtin_memcpy(w, p, BYTES); }
+    __device__ __forceinline__ void from_any(const T* p) {
+        if constexpr (BYTES < 4) from(p);
+        else __builtin_memcpy(w, p, BYTES);
+    }
     __device__ __forceinline__ void drop(int n) {
         static_assert(V == 4, "four elements");
         drop_first<T>(w, n);

@@ -607,8 +607,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int
             x[i].from((const T*)q.x + b * q.x_b + ec);
             dt[i].from((const T*)q.dt + b * q.dt_b + ec);
             z[i].from((const T*)q.z + b * q.z_b + ec);
-            bm[i].from((const T*)q.b + b * q.b_b + kc);
-            cm[i].from((const T*)q.c + b * q.c_b + kc);
+            bm[i].from_any((const T*)q.b + b * q.b_b + kc);
+            cm[i].from_any((const T*)q.c + b * q.c_b + kc);
         }
     }
 #pragma unroll
@@ -662,18 +662,109 @@ static int launch_steps(const ScanArgs& a, int batch, hipStream_t st) {
     return batch >= 4 && (int64_t)a.channels * a.n / V * batch >= 4 * 512 * kScanThreads ? launch_step<T, V, 4>(a, batch, st) : launch_step<T, V, 1>(a, batch, st);
 }
 
+// Few positions: as one position, P lanes for a channel with V adjacent states each, and all operands straight from memory, kNear positions
+// ahead: no tile to fill, no LDS that few workgroups of a CU share.  Measured, bf16, against the tiles: 100 sequences x 2048 channels x 16
+// states 14 us for 2 positions (33), 30 for 12 (37), 99 for 50 (87); x 64 states 36 for 2 (225), 172 for 24 (317); one sequence x 4096 x 16
+// 6 to 14 us up to 12 positions (7 to 9), 12 for 24 (7).
+constexpr int kNear = 4;
+
+template <class T, int P, int V>
+__global__ __launch_bounds__(kScanThreads) void scan_short_kernel(ScanArgs q) {
+    constexpr int CW = kScanThreads / P;
+    const int64_t id = block_index();
+    if (id >= q.blocks) return;
+    int64_t b;
+    int group;
+    q.by_groups.split(id, b, group);
+    const int tid = threadIdx.x, p = tid % P, E = q.channels, e = group * CW + tid / P, ec = min(e, E - 1), k = p * V, kc = min(k, q.n - V);
+    const bool mine = e < E && k < q.n;
+    const int n = q.lengths ? min(max(q.lengths[b], 0), q.len) : q.len;
+    const float bias = q.dt_bias ? q.dt_bias[ec] : 0.0f, dcoef = q.d ? q.d[ec] : 0.0f;
+    Pack<float, V> a = load<float, V>(q.a + (int64_t)ec * q.n + kc), h{};
+    if (q.state) h = load<float, V>(q.state + (b * E + ec) * q.n + kc);
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.v[j] *= kLog2e;
+    const T* x = (const T*)q.x + b * q.x_b + ec;
+    const T* dt = (const T*)q.dt + b * q.dt_b + ec;
+    const T* z = (const T*)q.z + b * q.z_b + ec;
+    const T* bm = (const T*)q.b + b * q.b_b + kc;
+    const T* cm = (const T*)q.c + b * q.c_b + kc;
+    T* y = (T*)q.y + b * q.len * (int64_t)E + e;
+    struct Rows {
+        Raw<T, 1> x[kNear], dt[kNear], z[kNear];
+        Raw<T, V> b[kNear], c[kNear];
+    } now, next;
+    auto fetch = [&](Rows& r, int t0) {          // rows behind the last valid one repeat it
+#pragma unroll
+        for (int i = 0; i < kNear; ++i) {
+            const int64_t t = min(t0 + i, n - 1);
+            r.x[i].from(x + t * q.x_r);
+            r.dt[i].from(dt + t * q.dt_r);
+            if (q.gate) r.z[i].from(z + t * q.z_r);
+            r.b[i].from_any(bm + t * q.b_r);
+            r.c[i].from_any(cm + t * q.c_r);
+        }
+    };
+    if (n > 0) fetch(now, 0);
+    for (int t0 = 0; t0 < n; t0 += kNear) {
+        if (t0 + kNear < n) fetch(next, t0 + kNear);
+#pragma unroll
+        for (int i = 0; i < kNear; ++i) {
+            if (t0 + i >= n) break;
+            float d = now.dt[i][0] + bias, out = 0.0f;
+            if (q.softplus) d = softplus(d);
+            const float dx = d * now.x[i][0];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h.v[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a.v[j]), h.v[j], dx * now.b[i][j]);
+                out = __builtin_fmaf(h.v[j], mine ? now.c[i][j] : 0.0f, out);
+            }
+            out = __builtin_fmaf(dcoef, now.x[i][0], lanes_sum<P>(out));
+            if (q.gate) out *= silu(now.z[i][0]);
+            if (p == 0 && e < E) y[(int64_t)(t0 + i) * E] = (T)out;
+        }
+        now = next;
+    }
+    if (e < E) {
+        for (int t = n + p; t < q.len; t += P) y[(int64_t)t * E] = (T)0.0f;
+        if (mine) store<float, V>(q.state_out + (b * E + e) * q.n + k, h);
+    }
+}
+
+template <class T, int V>
+static int launch_short(ScanArgs a, int64_t batch, hipStream_t st) {
+    int lanes = 1;
+    while (lanes * V < a.n) lanes *= 2;
+    const int64_t groups = ceil_div(a.channels, kScanThreads / lanes);
+    a.by_groups = Divisor(groups);
+    a.blocks = groups * batch;
+    if (a.blocks > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "selective_scan: the batch is too large for one call");
+    const dim3 grid = grid_of(a.blocks), block(kScanThreads);
+    switch (lanes) {
+        case 1: hipLaunchKernelGGL((scan_short_kernel<T, 1, V>), grid, block, 0, st, a); break;
+        case 2: hipLaunchKernelGGL((scan_short_kernel<T, 2, V>), grid, block, 0, st, a); break;
+        case 4: hipLaunchKernelGGL((scan_short_kernel<T, 4, V>), grid, block, 0, st, a); break;
+        case 8: hipLaunchKernelGGL((scan_short_kernel<T, 8, V>), grid, block, 0, st, a); break;
+        case 16: hipLaunchKernelGGL((scan_short_kernel<T, 16, V>), grid, block, 0, st, a); break;
+        case 32: hipLaunchKernelGGL((scan_short_kernel<T, 32, V>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((scan_short_kernel<T, 64, V>), grid, block, 0, st, a); break;
+    }
+    return TAE_OK;
+}
+
 // How a call is cut: lanes for a channel, each with per_lane states, and pieces along the positions.
 struct ScanPlan {
-    int lanes = 1, per_lane = 1, groups = 1, pieces = 1, piece_len = 0;
+    int lanes = 0, per_lane = 1, groups = 1, pieces = 1, piece_len = 0;       // lanes = 0: few positions, by scan_step_kernel or scan_short_kernel
     size_t steps_bytes = 0, bytes = 0;
 };
 
 constexpr int kPieceUnit = 64;                   // pieces are whole tiles
 
-// The ways to share a channel's states (4, 8, 16, 32 or 64 with those filled up) among lanes: by scan_lane_kernel with one lane, else by
-// selective_scan_kernel.  ns: what a wave takes for a position, with other waves on its SIMD; alone: the number of waves whose time one by
-// itself takes; start: us before a round of waves is under way.  Measured over lengths from 32 to 8192 and 128 to 131072 channels of all
-// sequences together, in bf16 with gate; what follows from them is within 16 % of the best of these ways and pieces.
+// The ways to share a channel's states (4, 8, 16, 32 or 64 with those filled up) among lanes: by scan_short_kernel (lanes = 0, four states
+// each), by scan_lane_kernel with one lane, else by selective_scan_kernel.  ns: what a wave takes for a position, with other waves on its
+// SIMD; alone: the number of waves whose time one by itself takes; start: us before a round of waves is under way, which up to 64
+// positions do not hide.  Measured over lengths from 2 to 8192 and 128 to 204800 channels of all sequences together, in bf16 with gate; what
+// follows from them is mostly within 16 % of the best of these ways and pieces, and within 9 us for few positions.
 //     us, pieces in (); batch x len x channels x states      1 lane      4 lanes     8 lanes     16 lanes
 //     1 x 4096 x 4096 x 16                                   146 (32)                136 (32)    163 (16)
 //     8 x 2048 x 1024 x 16                                   147 (16)                131 (8)     127 (1)
@@ -687,7 +778,9 @@ struct ScanForm {
     int lanes, per_lane;
     double ns, alone, start;
 };
-constexpr ScanForm kForms[] = {{4, 1, 71, 1.15, 0}, {8, 1, 31, 1.7, 0}, {1, 16, 285, 1.8, 2}, {8, 2, 49, 1.45, 0}, {16, 1, 31, 1.5, 0}, {8, 4, 75, 1.5, 0}, {16, 2, 45, 1.25, 0}, {16, 4, 96, 1.1, 0}};
+constexpr ScanForm kForms[] = {{0, 4, 232, 1.45, 1}, {0, 8, 180, 1.85, 1}, {0, 16, 152, 2.2, 1}, {0, 32, 130, 2.6, 1}, {0, 64, 138, 2.45, 1},
+                              {4, 1, 71, 1.15, 2}, {8, 1, 31, 1.7, 1}, {1, 16, 300, 1.8, 6}, {8, 2, 49, 1.45, 1}, {16, 1, 31, 1.5, 1.3}, {8, 4, 75, 1.5, 2},
+                              {16, 2, 45, 1.25, 2.5}, {16, 4, 96, 1.1, 4}};
 
 // Few channels leave SIMDs empty: then fewer states for each lane, or pieces along the positions, which cost a pass for their ends (0.6 of the
 // main one) and a launch that joins them (8 us).  The choice is the cheapest by these numbers and the waves that a SIMD (1024 of them) runs.
@@ -698,14 +791,15 @@ static bool plan_scan(const tae_scan_args* p, ScanPlan* out) {
     while (padded < p->states) padded *= 2;
     double least = 0.0;
     for (const ScanForm& f : kForms) {
-        if (f.lanes * f.per_lane != padded) continue;
-        const int64_t groups = ceil_div(p->channels, f.lanes == 1 ? 64 : kScanThreads / f.lanes), waves = f.lanes == 1 ? 1 : 4;
-        for (int64_t pieces = 1; pieces <= 64; ++pieces) {
+        const int share = f.lanes ? f.lanes : padded / 4;
+        if (f.per_lane * (f.lanes ? f.lanes : 1) != padded || (!f.lanes && p->len > 32)) continue;        // few positions: 32 at the most
+        const int64_t groups = ceil_div(p->channels, f.lanes == 1 ? 64 : kScanThreads / share), waves = f.lanes == 1 ? 1 : 4;
+        for (int64_t pieces = 1; pieces <= (f.lanes ? 64 : 1); ++pieces) {
             const int64_t piece_len = ceil_div(ceil_div(p->len, pieces), kPieceUnit) * kPieceUnit;
             if (ceil_div(p->len, piece_len) < pieces) continue;
             auto time = [&](int64_t n) {
                 const double all = std::ceil(n * waves * p->batch * groups / 1024.0 * 4.0) / 4.0;
-                return std::max(all, f.alone) * std::min<int64_t>(piece_len, p->len) * f.ns * 1e-3 + f.start * std::max(all, 1.0);
+                return std::max(all, f.alone) * std::min<int64_t>(piece_len, p->len) * f.ns * 1e-3 + (p->len <= 64 ? f.start * std::max(all, 1.0) : 0.0);
             };
             const double cost = time(pieces) + (pieces > 1 ? 0.6 * time(pieces - 1) + 8.0 : 0.0);
             if (least == 0.0 || cost < least) {
@@ -759,6 +853,7 @@ static int launch_lane(const ScanArgs& a, int64_t batch, hipStream_t st) {
 template <class T>
 static int launch_scan_plan(const ScanArgs& a, const ScanPlan& s, bool v, int batch, hipStream_t st) {
     if (a.len == 1) return v ? launch_steps<T, 4>(a, batch, st) : launch_steps<T, 1>(a, batch, st);
+    if (s.lanes == 0) return v ? launch_short<T, 4>(a, batch, st) : launch_short<T, 1>(a, batch, st);
     switch (s.lanes * 100 + s.per_lane) {
         case 116: return launch_lane<T, 16>(a, batch, st);
         case 401: return launch_scan<T, 1, 4, 32>(a, v, batch, st);
@@ -809,9 +904,7 @@ int tae_selective_scan(const tae_scan_args* p, void* stream) {
     if (p->z) w.elements(p->z_batch).elements(p->z_row);
     Width w4(4);
     w4.elements(p->states).pointer(p->a).pointer(p->state).pointer(p->state_out);
-    Width wb(dtype_bytes(p->dtype));
-    wb.pointer(p->b).pointer(p->c).elements(p->b_batch).elements(p->c_batch);
-    const bool vector = p->len > 1 ? w.fits(four) : w4.fits(16) && wb.fits(four);      // one position: of the states and of B and C
+    const bool vector = s.lanes ? w.fits(four) : w4.fits(16);         // loads of four channels; few positions: of four states
     if (a.blocks > ((int64_t)kGridX << 15)) return fail_msg(TAE_EINVAL, "selective_scan: the batch is too large for one call");
     return guarded([&] {
         hipStream_t st = (hipStream_t)stream;
