@@ -793,12 +793,13 @@ static bool plan_scan(const tae_scan_args* p, ScanPlan* out) {
     for (const ScanForm& f : kForms) {
         const int share = f.lanes ? f.lanes : padded / 4;
         if (f.per_lane * (f.lanes ? f.lanes : 1) != padded || (!f.lanes && p->len > 32)) continue;        // few positions: 32 at the most
-        const int64_t groups = ceil_div(p->channels, f.lanes == 1 ? 64 : kScanThreads / share), waves = f.lanes == 1 ? 1 : 4;
+        const int64_t groups = ceil_div(p->channels, f.lanes == 1 ? 64 : kScanThreads / share);
         for (int64_t pieces = 1; pieces <= (f.lanes ? 64 : 1); ++pieces) {
             const int64_t piece_len = ceil_div(ceil_div(p->len, pieces), kPieceUnit) * kPieceUnit;
             if (ceil_div(p->len, piece_len) < pieces) continue;
             auto time = [&](int64_t n) {
-                const double all = std::ceil(n * waves * p->batch * groups / 1024.0 * 4.0) / 4.0;
+                const double cus = ceil_div(n * p->batch * groups, f.lanes == 1 ? kLaneWaves : 1) / 256.0;         // workgroups for each
+                const double all = f.lanes == 1 ? 2.0 * std::ceil(cus) : cus < 4.0 ? std::ceil(cus) : cus;          // waves for a SIMD of the fullest
                 return std::max(all, f.alone) * std::min<int64_t>(piece_len, p->len) * f.ns * 1e-3 + (p->len <= 64 ? f.start * std::max(all, 1.0) : 0.0);
             };
             const double cost = time(pieces) + (pieces > 1 ? 0.6 * time(pieces - 1) + 8.0 : 0.0);
