@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 FORMS = [(5, 5, 19757, 1), (1, 421, 14432, 1), (5, 5, 19756, 5), (1, 700, 9011, 5), (5, 5, 19757, 9), (5, 5, 19756, 17), (5, 700, 1602, 5), (3, 5, 16885, 9), (1, 700, 4808, 9),
          (3, 5, 16885, 17), (3, 5, 16885, 33), (2, 700, 2193, 9), (2, 5, 12335, 17), (1, 700, 2566, 17), (1, 5, 12335, 33), (1, 500, 3512, 33), (3, 5, 16884, 1), (1, 421, 7701, 1),
          (3, 5, 16885, 5), (1, 500, 6582, 5), (2, 5, 12335, 5), (1, 421, 3512, 5), (2, 5, 12336, 9), (1, 500, 3512, 9), (1, 300, 1, 5), (1, 5, 12335, 9), (1, 421, 1874, 9), (1, 5, 12335, 17),
-         (1, 421, 1874, 17), (1, 300, 4, 9), (1, 300, 3, 17), (1, 300, 1, 64), (5, 50, 19757, 9), (1, 2100, 4100, 9), (1, 421, 1369, 9), (1, 421, 1602, 17),
+         (1, 421, 1874, 17), (1, 300, 4, 9), (1, 300, 3, 17), (1, 300, 1, 64), (5, 50, 19757, 9), (1, 2100, 4100, 9), (1, 2048, 4096, 9), (12, 12, 10543, 9), (1, 421, 1369, 9), (1, 421, 1602, 17),
          (1, 20, 4000, 3), (1, 20, 12335, 5), (2, 20, 12335, 9), (1, 20, 300, 9), (1, 20, 12335, 17), (1, 20, 300, 17), (1, 30, 3000, 33), (3, 7, 100, 64), (2, 12, 65, 4), (3, 2, 33, 16),
          (2, 24, 40, 64), (4, 9, 3, 2), (2, 3, 1, 1)]
 
