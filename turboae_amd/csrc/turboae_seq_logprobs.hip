@@ -175,8 +175,12 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
     again();
     const int wave = threadIdx.x >> 6;
     float mine = kNegInf, of[G];                 // largest of the lane and of its granules; NaN if there is one
+    // granules behind the row for a whole wave are left out
+    auto filled = [&](int g) { return W < 64 || __builtin_amdgcn_readfirstlane(place(g)) < hi; };
 #pragma unroll
     for (int g = 0; g < G; ++g) {
+        of[g] = kNegInf;
+        if (!filled(g)) continue;
         of[g] = value(g, 0);
 #pragma unroll
         for (int i = 1; i < V; ++i) of[g] = __builtin_elementwise_maximum(of[g], value(g, i));
@@ -228,13 +232,15 @@ __global__ __launch_bounds__(THREADS) void logprobs_part_kernel(LogprobsArgs a) 
     float s = 0.0f, t = 0.0f;
     auto sums = [&](auto&& distance) {
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+            if (!filled(g)) continue;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float d = fmaxf(distance(value(g, i)), -1000.0f), e = __builtin_amdgcn_exp2f(d);
                 s += e;
                 t = __builtin_fmaf(d, e, t);
             }
+        }
     };
     if (near) sums([&](float x) { return __builtin_fmaf(x, kLog2e, -c); });
     else sums([&](float x) { return (x - base) * kLog2e; });
