@@ -1,0 +1,39 @@
+"""What turboae_amd.sequence refuses before the library is called, seen without a GPU: tensors that say they are on one, so that a call
+gets as far as it would there.  One that is let through fails on the missing device instead."""
+import pytest
+import torch
+
+from turboae_amd import sequence
+
+
+class OnDevice(torch.Tensor):
+    is_cuda = True
+
+
+def dev(t):
+    return t.as_subclass(OnDevice)
+
+
+def many(n, *shape, dtype=torch.float32):
+    """A tensor of n equal parts without memory for them."""
+    return dev(torch.zeros(1, *shape, dtype=dtype).expand(n, *shape))
+
+
+PAST = (1 << 32) + 1                             # 1 in the library's 32-bit sizes
+
+
+@pytest.mark.parametrize("call", [
+    lambda n: sequence.causal_conv(many(n, 1, 1), dev(torch.zeros(1, 2))),
+    lambda n: sequence.causal_conv(dev(torch.zeros(1, 1, 1).expand(1, n, 1)), dev(torch.zeros(1, 2))),
+    lambda n: sequence.selective_scan(many(n, 1, 1), many(n, 1, 1), dev(-torch.ones(1, 1)), many(n, 1, 1), many(n, 1, 1)),
+    lambda n: sequence.norm_residual(many(n, 1, 4), pre_weight=dev(torch.ones(4)), dtype=torch.float32),
+    lambda n: sequence.quantize_int8(many(n, 4)),
+    lambda n: sequence.int8_linear(many(n, 16), dev(torch.zeros(1, 16, dtype=torch.int8)), dev(torch.ones(1))),
+    lambda n: sequence.int8_linear(dev(torch.zeros(1, 16)), dev(torch.zeros(1, 16, dtype=torch.int8).expand(n, 16)), dev(torch.ones(1).expand(n))),
+    lambda n: sequence.token_logprobs(many(n, 1), dev(torch.zeros(1, dtype=torch.int32).expand(n))),
+])
+@pytest.mark.parametrize("n", [PAST, 1 << 31])
+def test_sizes_past_32_bits_are_refused(call, n):
+    """They would be cut to their low 32 bits on the way to the library, and most of the outputs left as they were allocated."""
+    with pytest.raises(ValueError, match="2\\^31"):
+        call(n)

@@ -15,7 +15,8 @@ No reference counterpart.
 Activations are float32, float16 or bfloat16, (batch, len, channels) with adjacent channels - a slice of a wider tensor is taken as it is,
 without a copy; parameters and states named float32 are float32.  Sums, norms, softmax statistics and states are kept in 32 bits or more
 and each result is rounded once.  ``lengths`` (int32, one for each sequence) marks padding: positions at or behind it are not read, their
-outputs are zero, and the state is the one after the last position in front of them.
+outputs are zero, and the state is the one after the last position in front of them.  Sizes, rows of all leading dimensions together among
+them, are below 2^31.
 """
 from __future__ import annotations
 
@@ -46,6 +47,11 @@ class _Call:
         if first.dtype not in _DTYPE:
             raise ValueError(f"{name}: float32, float16 or bfloat16 wanted, got {first.dtype}")
         self.name, self.device, self.dtype, self.grad, self.new = name, first.device, first.dtype, torch.is_grad_enabled(), first.new_empty
+
+    def sizes(self, *sizes: int) -> None:
+        """The library's sizes have 32 bits, and ctypes would cut larger ones to them."""
+        if max(sizes) > 0x7FFFFFFF:
+            raise ValueError(f"{self.name}: sizes must be below 2^31, got {sizes}")
 
     def tensor(self, t: Optional[torch.Tensor], what: str, shape: Tuple[int, ...], dtype: torch.dtype, dense: bool = False) -> Optional[int]:
         """Address of a tensor after its checks (None for None): shape, type, device, adjacent last elements; dense: contiguous."""
@@ -89,9 +95,10 @@ class _Call:
             _lib.check(rc)
 
 
-def _sequence(name: str, what: str, t: torch.Tensor) -> Tuple[int, int, int]:
+def _sequence(c: _Call, what: str, t: torch.Tensor) -> Tuple[int, int, int]:
     if t.dim() != 3 or t.numel() == 0:
-        raise ValueError(f"{name}: {what} must have shape (batch, len, channels), none of them 0, got {tuple(t.shape)}")
+        raise ValueError(f"{c.name}: {what} must have shape (batch, len, channels), none of them 0, got {tuple(t.shape)}")
+    c.sizes(*t.shape)
     return t.shape
 
 
@@ -124,7 +131,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     (batch, taps - 1, channels) of x's type: the last inputs of an earlier call, oldest first (None: zeros).  Returns (y, the state after
     this call); with one position this is the single-token step.  ``state_out`` receives the state and may be ``state`` itself."""
     c = _Call("causal_conv", x)
-    B, L, E = _sequence(c.name, "x", x)
+    B, L, E = _sequence(c, "x", x)
     if weight.dim() != 2:
         raise ValueError(f"causal_conv: weight must have shape (channels, taps), got {tuple(weight.shape)}")
     K = weight.shape[1]
@@ -155,7 +162,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     (channels) and ``state`` (batch, channels, states; None: zeros) float32.  Returns (y, the state after the last position); with one
     position this is the single-token step.  ``state_out`` receives the state and may be ``state`` itself."""
     c = _Call("selective_scan", x)
-    b, L, E = _sequence(c.name, "x", x)
+    b, L, E = _sequence(c, "x", x)
     if A.dim() != 2 or not 1 <= A.shape[1] <= 64:
         raise ValueError(f"selective_scan: A must have shape (channels, states) with 1 to 64 states, got {tuple(A.shape)}")
     N = A.shape[1]
@@ -192,7 +199,7 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
     float32; scale, weights and biases (dim) float32.  Without a block r is the residual, and ``dtype`` names normed's type (None: the
     residual's).  Returns (r, normed); ``residual_out`` receives r and may be ``residual`` itself."""
     c = _Call("norm_residual", residual if block is None else block)
-    B, L, D = _sequence(c.name, "residual", residual)
+    B, L, D = _sequence(c, "residual", residual)
     f32 = torch.float32
     if block is None and dtype is not None:
         if dtype not in _DTYPE:
@@ -238,6 +245,7 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if x.dim() != 2 or 0 in x.shape:
         raise ValueError(f"quantize_int8: x must have shape (rows, columns), none of them 0, got {tuple(x.shape)}")
     R, K = x.shape
+    c.sizes(R, K)
     address = c.tensor(x, "x", (R, K), c.dtype)
     step = -(-K // 64) * 64
     q = c.new((R, step), dtype=torch.int8)
@@ -254,8 +262,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if x.dim() < 1 or 0 in x.shape or weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"int8_linear: x (..., inputs) and weight (outputs, inputs) wanted, none of them 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
     N, K = weight.shape
+    M = x.numel() // x.shape[-1]
+    c.sizes(M, N)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    M = rows.shape[0]
     if K > 131072:
         raise ValueError(f"int8_linear: at most 131072 inputs, got {K}")
     c.tensor(rows, "x", (M, K), c.dtype)
@@ -288,8 +297,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     V = logits.shape[-1]
     if not 0 <= top <= min(32, V) or V > 1 << 21:
         raise ValueError(f"token_logprobs: top must be in 0..32 and at most vocab, vocab at most 2^21, got {top} of {V}")
+    R = logits.numel() // V
+    c.sizes(R)
     flat = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    R = flat.shape[0]
     shape = tuple(tokens.shape)
     logp = c.new(shape, dtype=torch.float32)
     entropy = c.new(shape, dtype=torch.float32)
