@@ -37,3 +37,10 @@ def test_sizes_past_32_bits_are_refused(call, n):
     """They would be cut to their low 32 bits on the way to the library, and most of the outputs left as they were allocated."""
     with pytest.raises(ValueError, match="2\\^31"):
         call(n)
+
+
+def test_a_type_that_a_block_overrides_is_refused():
+    """normed has the block's type; another one that is asked for beside it is not passed over."""
+    r, b, w = dev(torch.zeros(1, 2, 4)), dev(torch.zeros(1, 2, 4, dtype=torch.bfloat16)), dev(torch.ones(4))
+    with pytest.raises(ValueError, match="block"):
+        sequence.norm_residual(r, b, pre_weight=w, dtype=torch.float32)

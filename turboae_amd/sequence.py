@@ -197,7 +197,7 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
     ``norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps)``, mean 0 unless center.  residual, block (batch, len, dim); gate of that
     shape or (batch, 1, dim), one for each sequence; gate_act "linear", "tanh", "sigmoid" or "silu"; the residual has the block's type or
     float32; scale, weights and biases (dim) float32.  Without a block r is the residual, and ``dtype`` names normed's type (None: the
-    residual's).  Returns (r, normed); ``residual_out`` receives r and may be ``residual`` itself."""
+    residual's); with one it has the block's.  Returns (r, normed); ``residual_out`` receives r and may be ``residual`` itself."""
     c = _Call("norm_residual", residual if block is None else block)
     B, L, D = _sequence(c, "residual", residual)
     f32 = torch.float32
@@ -205,6 +205,8 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
         if dtype not in _DTYPE:
             raise ValueError(f"norm_residual: dtype must be float32, float16 or bfloat16, got {dtype}")
         c.dtype = dtype
+    elif dtype is not None and dtype is not c.dtype:
+        raise ValueError(f"norm_residual: with a block normed has its type, {c.dtype}, got dtype {dtype}")
     if residual.dtype not in (c.dtype, f32):
         raise ValueError(f"norm_residual: the residual has the block's type or float32, got {residual.dtype} beside {c.dtype}")
     if gate_act not in _ACT:
