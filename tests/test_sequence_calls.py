@@ -2,6 +2,7 @@
 gets as far as it would there.  One that is let through fails on the missing device instead."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from turboae_amd import sequence
 
@@ -44,3 +45,26 @@ def test_a_type_that_a_block_overrides_is_refused():
     r, b, w = dev(torch.zeros(1, 2, 4)), dev(torch.zeros(1, 2, 4, dtype=torch.bfloat16)), dev(torch.ones(4))
     with pytest.raises(ValueError, match="block"):
         sequence.norm_residual(r, b, pre_weight=w, dtype=torch.float32)
+
+
+X, W, ONES = dev(torch.zeros(1, 2, 16)), dev(torch.zeros(16, 4)), dev(torch.ones(16))
+A, BC = dev(-torch.ones(16, 8)), dev(torch.zeros(1, 2, 8))
+Q, T = dev(torch.zeros(4, 16, dtype=torch.int8)), dev(torch.zeros(2, dtype=torch.int64))
+
+
+def dual(t):
+    return dev(forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+@pytest.mark.parametrize("call", [
+    lambda d: sequence.causal_conv(d(X), W), lambda d: sequence.causal_conv(X, W, d(ONES)), lambda d: sequence.causal_conv(X, W, state_out=d(dev(torch.zeros(1, 3, 16)))),
+    lambda d: sequence.selective_scan(X, d(X), A, BC, BC), lambda d: sequence.selective_scan(X, X, A, BC, BC, z=d(X)), lambda d: sequence.selective_scan(X, X, d(A), BC, BC),
+    lambda d: sequence.norm_residual(d(X), X), lambda d: sequence.norm_residual(X, X, gate=d(X)), lambda d: sequence.norm_residual(X, X, residual_out=d(dev(torch.zeros(1, 2, 16)))),
+    lambda d: sequence.quantize_int8(d(X[0])), lambda d: sequence.int8_linear(d(X), Q, ONES[:4]), lambda d: sequence.int8_linear(X, Q, ONES[:4], bias=d(ONES[:4])),
+    lambda d: sequence.token_logprobs(d(X[0]), T),
+])
+def test_forward_mode_tangents_are_refused(call):
+    """A dual tensor does not require a gradient; without a refusal the call would return values whose tangents are gone."""
+    with forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(ValueError, match="tangent"):
+            call(dual)

@@ -9,8 +9,8 @@
 They stand beside ``Channel_AE_HIP`` as the recurrent and convolution stacks, the power norm, the precisions and ``count_errors`` do
 inside it, and follow its manner: all arithmetic runs in libturboae_hip.so on tensors of a ROCm device (no CPU fallback), a call enqueues
 work on the current stream of its tensors' device and never synchronises, and wrong shapes, types, devices or layouts raise ``ValueError``
-before anything is launched.  The path is inference: a tensor that requires a gradient is refused (call under ``torch.no_grad()``).
-No reference counterpart.
+before anything is launched.  The path is inference: a tensor that requires a gradient is refused (call under ``torch.no_grad()``),
+and so is one with a forward-mode tangent.  No reference counterpart.
 
 Activations are float32, float16 or bfloat16, (batch, len, channels) with adjacent channels - a slice of a wider tensor is taken as it is,
 without a copy; parameters and states named float32 are float32.  Sums, norms, softmax statistics and states are kept in 32 bits or more
@@ -24,6 +24,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -39,7 +40,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 class _Call:
     """The checks that every tensor of a call goes through, against the first of them; a call of a single token costs little more."""
 
-    __slots__ = ("name", "device", "dtype", "grad", "new")
+    __slots__ = ("name", "device", "dtype", "grad", "tangents", "new")
 
     def __init__(self, name: str, first: torch.Tensor):
         if not isinstance(first, torch.Tensor) or not first.is_cuda:
@@ -47,6 +48,7 @@ class _Call:
         if first.dtype not in _DTYPE:
             raise ValueError(f"{name}: float32, float16 or bfloat16 wanted, got {first.dtype}")
         self.name, self.device, self.dtype, self.grad, self.new = name, first.device, first.dtype, torch.is_grad_enabled(), first.new_empty
+        self.tangents = getattr(forward_ad, "_current_level", 0) >= 0              # inside a dual_level, the only place for tangents
 
     def sizes(self, *sizes: int) -> None:
         """The library's sizes have 32 bits, and ctypes would cut larger ones to them."""
@@ -66,6 +68,8 @@ class _Call:
                 raise ValueError(f"{self.name}: adjacent elements of {what}'s last dimension must be adjacent in memory")
         if self.grad and t.requires_grad:
             raise ValueError(f"{self.name}: {what} requires a gradient, but this path is inference only (call it under torch.no_grad())")
+        if self.tangents and forward_ad.unpack_dual(t).tangent is not None:      # torch.no_grad() does not turn tangents off
+            raise ValueError(f"{self.name}: {what} has a forward-mode tangent, but this path is inference only (call it with unpack_dual's primal)")
         return t.data_ptr()
 
     def out(self, t: Optional[torch.Tensor], what: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
