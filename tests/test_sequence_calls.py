@@ -68,3 +68,33 @@ def test_forward_mode_tangents_are_refused(call):
     with forward_ad.dual_level(), torch.no_grad():
         with pytest.raises(ValueError, match="tangent"):
             call(dual)
+
+
+@pytest.mark.parametrize("call,shape", [
+    (lambda out: sequence.causal_conv(X, W, state_out=out), (1, 3, 16)), (lambda out: sequence.causal_conv(X, W, state=out, state_out=out), (1, 3, 16)),
+    (lambda out: sequence.selective_scan(X, X, A, BC, BC, state=out, state_out=out), (1, 16, 8)),
+    (lambda out: sequence.norm_residual(X, X, residual_out=out), (1, 2, 16)), (lambda out: sequence.norm_residual(out, X, residual_out=out), (1, 2, 16)),
+    (lambda out: sequence.norm_residual(X, pre_weight=ONES, residual_out=out), (1, 2, 16)),
+])
+def test_what_is_written_in_place_is_seen_by_autograd(monkeypatch, call, shape):
+    """An older graph that has saved the tensor says so in its backward pass, as after any operation in place."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(sequence, "_raw_stream", lambda index: None)
+    for name in ("tae_causal_conv", "tae_selective_scan", "tae_norm_residual"):
+        monkeypatch.setattr(sequence._lib.load(), name, lambda *args: 0)
+    out, w = dev(torch.ones(shape)), torch.ones(shape, requires_grad=True)
+    saved = (w * out.as_subclass(torch.Tensor)).sum()
+    call(out)
+    with pytest.raises(RuntimeError, match="inplace"):
+        saved.backward()
+
+
+def test_a_tensor_that_is_only_read_keeps_its_version(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(sequence, "_raw_stream", lambda index: None)
+    monkeypatch.setattr(sequence._lib.load(), "tae_norm_residual", lambda *args: 0)
+    r = dev(torch.ones(1, 2, 16))
+    assert sequence.norm_residual(r, pre_weight=ONES)[0] is r and r._version == 0
+    assert sequence.norm_residual(r, pre_weight=ONES, residual_out=r)[0] is r and r._version == 0
+    sequence.norm_residual(r, r, pre_weight=ONES)
+    assert r._version == 0

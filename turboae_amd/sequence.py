@@ -25,6 +25,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -88,7 +89,8 @@ class _Call:
         args.workspace, args.workspace_bytes = w.data_ptr(), n
         return w
 
-    def run(self, entry, *args) -> None:
+    def run(self, entry, *args, writes: Optional[torch.Tensor] = None) -> None:
+        """`writes`: a tensor of the caller that the call changes; autograd sees it as after any operation in place."""
         index = self.device.index
         if torch.cuda.current_device() == index:
             rc = entry(*args, _raw_stream(index))
@@ -97,6 +99,8 @@ class _Call:
                 rc = entry(*args, _raw_stream(index))
         if rc:
             _lib.check(rc)
+        if writes is not None:
+            increment_version(writes)
 
 
 def _sequence(c: _Call, what: str, t: torch.Tensor) -> Tuple[int, int, int]:
@@ -145,12 +149,12 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     y = c.new((B, L, E), dtype=c.dtype)
     if state_out is not None and K > 1:
         _in_place_or_apart(c.name, state_out, state, x, weight, bias, lengths)
-    state_out = c.out(state_out, "state_out", (B, K - 1, E), c.dtype)
+    given, state_out = state_out, c.out(state_out, "state_out", (B, K - 1, E), c.dtype)
     args = _lib.TaeConvArgs(ctypes.sizeof(_lib.TaeConvArgs), _DTYPE[c.dtype], B, L, E, K, _ACT[act], 0, x.stride(0), x.stride(1),
                             c.tensor(x, "x", (B, L, E), c.dtype), c.tensor(weight, "weight", (E, K), f32, True), c.tensor(bias, "bias", (E,), f32, True),
                             c.tensor(state, "state", (B, K - 1, E), c.dtype, True) if K > 1 else None,
                             c.tensor(lengths, "lengths", (B,), torch.int32, True), y.data_ptr(), state_out.data_ptr() if K > 1 else None)
-    c.run(_lib.load().tae_causal_conv, ctypes.byref(args))
+    c.run(_lib.load().tae_causal_conv, ctypes.byref(args), writes=given)
     return y, state_out
 
 
@@ -174,7 +178,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     y = c.new((b, L, E), dtype=c.dtype)
     if state_out is not None:
         _in_place_or_apart(c.name, state_out, state, x, dt, A, B, C, D, z, dt_bias, lengths)
-    state_out = c.out(state_out, "state_out", (b, E, N), f32)
+    given, state_out = state_out, c.out(state_out, "state_out", (b, E, N), f32)
     args = _lib.TaeScanArgs(ctypes.sizeof(_lib.TaeScanArgs), _DTYPE[c.dtype], b, L, E, N, 1 if softplus else 0, 0,
                             *_strides(x), *_strides(dt), *_strides(B), *_strides(C), *_strides(z),
                             c.tensor(x, "x", (b, L, E), c.dtype), c.tensor(dt, "dt", (b, L, E), c.dtype), c.tensor(A, "A", (E, N), f32, True),
@@ -184,7 +188,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
                             y.data_ptr(), state_out.data_ptr(), None, 0)
     lib = _lib.load()
     w = c.workspace(args, lib.tae_selective_scan_workspace)  # noqa: F841
-    c.run(lib.tae_selective_scan, ctypes.byref(args))
+    c.run(lib.tae_selective_scan, ctypes.byref(args), writes=given)
     return y, state_out
 
 
@@ -239,7 +243,7 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
                             *_strides(residual), *_strides(block), *ga, *_strides(out), c.tensor(residual, "residual", (B, L, D), residual.dtype),
                             c.tensor(block, "block", (B, L, D), c.dtype), None if gate is None else gate.data_ptr(), *vectors,
                             out.data_ptr() if write else None, None if normed is None else normed.data_ptr())
-    c.run(_lib.load().tae_norm_residual, ctypes.byref(args))
+    c.run(_lib.load().tae_norm_residual, ctypes.byref(args), writes=residual_out if write else None)
     return out, normed
 
 
