@@ -4,7 +4,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from turboae_amd import sequence
+from tests import test_sequence_cpu as C
+from turboae_amd import _lib, sequence
 
 
 class OnDevice(torch.Tensor):
@@ -98,3 +99,8 @@ def test_a_tensor_that_is_only_read_keeps_its_version(monkeypatch):
     assert sequence.norm_residual(r, pre_weight=ONES, residual_out=r)[0] is r and r._version == 0
     sequence.norm_residual(r, r, pre_weight=ONES)
     assert r._version == 0
+
+
+@pytest.mark.parametrize("make,entry", [(C.conv, "tae_causal_conv"), (C.scan, "tae_selective_scan"), (C.int8, "tae_int8_linear")])
+def test_reserved_fields_have_to_be_zero(make, entry):
+    C.refused(getattr(_lib.load(), entry), make(), "reserved", reserved=1)

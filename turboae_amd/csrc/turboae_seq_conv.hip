@@ -136,6 +136,7 @@ extern "C" int tae_causal_conv(const tae_conv_args* p, void* stream) {
     using namespace tae;
     using namespace tae::seq;
     if (!p || p->struct_size != (int32_t)sizeof(tae_conv_args)) return fail_msg(TAE_EINVAL, "tae_conv_args: NULL or struct_size mismatch (ABI)");
+    if (p->reserved) return fail_msg(TAE_EINVAL, "causal_conv: reserved must be 0");
     if (!dtype_ok(p->dtype)) return fail_msg(TAE_EINVAL, "causal_conv: dtype must be a TAE_DTYPE_* code");
     if (p->batch < 1 || p->len < 1 || p->channels < 1) return fail_msg(TAE_EINVAL, "causal_conv: batch, len and channels must be >= 1");
     if (p->len > INT32_MAX - 64 || p->channels > INT32_MAX - 64) return fail_msg(TAE_EINVAL, "causal_conv: len and channels must stay below 2^31 - 64");

@@ -627,6 +627,7 @@ int tae_int8_linear(const tae_int8_args* p, void* stream) {
     using namespace tae;
     using namespace tae::seq;
     if (!p || p->struct_size != (int32_t)sizeof(tae_int8_args)) return fail_msg(TAE_EINVAL, "tae_int8_args: NULL or struct_size mismatch (ABI)");
+    if (p->reserved) return fail_msg(TAE_EINVAL, "int8_linear: reserved must be 0");
     if (!dtype_ok(p->dtype)) return fail_msg(TAE_EINVAL, "int8_linear: dtype must be a TAE_DTYPE_* code");
     if (!int8_sizes(p)) return fail_msg(TAE_EINVAL, "int8_linear: inputs must be in 1..131072, rows and outputs in 1..2^30");
     if (!p->x || !p->weight || !p->weight_scale || !p->y) return fail_msg(TAE_EINVAL, "int8_linear: x, weight, weight_scale and y must not be NULL");

@@ -884,6 +884,7 @@ int tae_selective_scan(const tae_scan_args* p, void* stream) {
     using namespace tae;
     using namespace tae::seq;
     if (!p || p->struct_size != (int32_t)sizeof(tae_scan_args)) return fail_msg(TAE_EINVAL, "tae_scan_args: NULL or struct_size mismatch (ABI)");
+    if (p->reserved) return fail_msg(TAE_EINVAL, "selective_scan: reserved must be 0");
     if (!dtype_ok(p->dtype)) return fail_msg(TAE_EINVAL, "selective_scan: dtype must be a TAE_DTYPE_* code");
     if (p->states < 1 || p->states > 64) return fail_msg(TAE_EINVAL, "selective_scan: states must be in 1..64");
     if (p->batch < 1 || p->len < 1 || p->channels < 1) return fail_msg(TAE_EINVAL, "selective_scan: batch, len and channels must be >= 1");
