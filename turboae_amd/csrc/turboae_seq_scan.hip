@@ -427,12 +427,16 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
             r.bc[j].from(row, k, q.n);
         }
     };
+    // Lanes read what others of the wave wrote.  Its LDS instructions are carried out in the order of the program; the fences, no instructions
+    // themselves, keep that order the one written here: reads of this buffer's last use, writes, reads.
     auto stage = [&](const Raw& r, int buf) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
             const int i = j * 64 + lane;
             if (kAhead * W % 64 == 0 || i < kAhead * W) rows[buf][i] = i % N < q.n ? r.bc[j][0] : 0.0f;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
     Raw now, next;
 #pragma unroll
