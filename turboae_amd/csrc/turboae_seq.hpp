@@ -9,7 +9,7 @@
 #include <exception>
 #include <type_traits>
 
-#include "../../include/turboae_hip.h"
+#include "turboae_seq_plan.hpp"
 
 namespace tae {
 
@@ -133,15 +133,11 @@ __device__ __forceinline__ float lanes_max(float v) {
     return lanes_join<W>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-inline size_t dtype_bytes(int32_t t) { return t == TAE_DTYPE_F32 ? 4 : 2; }
-inline bool dtype_ok(int32_t t) { return t >= TAE_DTYPE_F32 && t <= TAE_DTYPE_BF16; }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 // every pointer on a multiple of its elements' size (NULL is)
 template <class... P>
 inline bool elements_aligned(size_t n, const P*... p) { return (aligned(p, n) && ...); }
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// Largest V of {16 / size, 4 / size, 1} that divides every given size and stride and to which every pointer is aligned.
+// How wide loads and stores may be: collects sizes, strides and addresses; fits(n) says whether all of them are multiples of n bytes.
 struct Width {
     size_t bytes;
     int64_t all = 0;                             // bits of every size, stride (in elements) and address

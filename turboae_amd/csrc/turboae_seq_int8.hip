@@ -439,7 +439,6 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
 // 1024 5.8 and 9.8 us (7.5 and 13.9), 1 x 4096 x 4096 7.7 and 9.7 (9.0 and 14.4), 4 x 4096 x 4096 9.3 and 9.8 (9.6 and 14.6).  More rows or
 // inputs take longer to quantise again and again than a launch (with 8 groups a lane, 8 x 4096 x 4096: 16.1 where two launches take 9.9), and
 // so do more workgroups than the CUs hold at once (1 x 1024 x 51200: 33 where two take 16).
-constexpr int kRowsGroups = 4;                   // groups of 16 bytes that a lane holds
 template <class T>
 __global__ __launch_bounds__(512) void int8_rows_kernel(Int8Args a, const T* x, int64_t x_r, int share) {
     constexpr int V = 16 / sizeof(T), DEEP = 8;
@@ -542,43 +541,16 @@ static hipError_t launch_few(Int8Args a, hipStream_t st) {
     return hipSuccess;
 }
 
-// Which form.  Up to 256 tiles of 128 x 128 the cheapest by what whole calls measured in bf16, in us, kk = inputs / 4096 and r rounds of 256
-// workgroups (1 at least):
-//     few, 16 x 16 a workgroup   5.2 + 1.2 kk + r max(3.5, 3.7 kk)        few, 64 x 32   6.0 + 1.2 kk + r max(4.2, 11.4 kk)
-//     few, 32 x 32               5.2 + 1.2 kk + r max(3.0, 7.2 kk)        tiles          8.0 + 15.6 kk
-// off by a tenth at most from 512 to 16384 inputs, 64 to 16384 outputs and 16 to 512 rows.  Among them, with 4096 outputs:
-//     4096 inputs, rows    16   32   64  128  256  512          16384 inputs, rows   16   32   64  128  256  512
-//     16 x 16              10   14   22   38   69  131                               27   42   71  127  236  458
-//     32 x 32              12   14   14   22   36   66                               38   41   42   70  126  239
-//     64 x 32              14   16   18   19   30   53                               43   48   56   57  100  185
-//     tiles                22   23   22   23   24   26                               71   71   71   71   72   76
-// More tiles:
-//     4096 inputs and outputs, rows                        1024  2048  3000  4096          8000 rows, 4000 outputs, inputs  200  500 1000 2000
-//     128 x 128, four buffers                                30    51    72    98                                            41   53   70  107
-//     the same, two buffers, two workgroups for a CU         34    46    67    91                                            35   47   63   96
-//     256 x 256                                                    57    63    83                                            57   65   78  101
 template <class T>
-static hipError_t launch_int8(const Int8Args& a, hipStream_t st) {
-    const int64_t large = ceil_div(a.m, 256) * ceil_div(a.n, 256), small = ceil_div(a.m, 128) * ceil_div(a.n, 128);
-    if (large >= 192 && a.k >= 4096) return launch_tiles<T, 256, 256, 2, 4, 2>(a, st);
-    if (small > 256) return launch_tiles<T, 128, 128, 2, 2, 2>(a, st);
-    const double kk = a.k / 4096.0;
-    auto rounds = [&](int rows, int outputs) { return std::max(1.0, ceil_div(a.m, rows) * ceil_div(a.n, outputs) / 256.0); };
-    const double by16 = 5.2 + 1.2 * kk + rounds(16, 16) * std::max(3.5, 3.7 * kk), by32 = 5.2 + 1.2 * kk + rounds(32, 32) * std::max(3.0, 7.2 * kk);
-    const double by64 = 6.0 + 1.2 * kk + rounds(64, 32) * std::max(4.2, 11.4 * kk), tiles = 8.0 + 15.6 * kk, least = std::min({by16, by32, by64, tiles});
-    if (least == by16) return launch_few<T, 1, 1, 8>(a, st);
-    if (least == by32) return launch_few<T, 2, 2, 4>(a, st);
-    if (least == by64) return launch_few<T, 4, 2, 4>(a, st);
-    return launch_tiles<T, 128, 128, 2, 2, 4>(a, st);
-}
-
-// Whether int8_rows_kernel takes a call: its rows fit the registers of a workgroup (and so LDS, 16 bytes off multiples of 64 so that the rows
-// meet all banks), and the workgroups that repeat the quantising are few.
-constexpr int64_t kRowsBlocks = 512;
-static int rows_share(const tae_int8_args* p) { return p->rows == 1 ? 8 : p->rows == 2 ? 4 : p->rows <= 4 ? 2 : 1; }
-static bool int8_in_one(const tae_int8_args* p) {
-    const int64_t across = 64 * 16 / (int64_t)dtype_bytes(p->dtype) * rows_share(p);
-    return p->rows <= 8 && p->inputs <= across * kRowsGroups && ceil_div(p->outputs, 16) <= kRowsBlocks;
+static hipError_t launch_int8(const Int8Args& a, Int8Form form, hipStream_t st) {
+    switch (form) {
+        case Int8Form::tiles256: return launch_tiles<T, 256, 256, 2, 4, 2>(a, st);
+        case Int8Form::tiles128_two: return launch_tiles<T, 128, 128, 2, 2, 2>(a, st);
+        case Int8Form::few16: return launch_few<T, 1, 1, 8>(a, st);
+        case Int8Form::few32: return launch_few<T, 2, 2, 4>(a, st);
+        case Int8Form::few64: return launch_few<T, 4, 2, 4>(a, st);
+        default: return launch_tiles<T, 128, 128, 2, 2, 4>(a, st);
+    }
 }
 
 template <class T>
@@ -592,10 +564,6 @@ static void launch_rows(Int8Args a, const tae_int8_args* p, hipStream_t st) {
 static int64_t q_stride(int32_t k) {
     const int64_t r = ceil_div(k, 128) * 128;
     return r % 1024 ? r : r + 128;
-}
-
-static bool int8_sizes(const tae_int8_args* p) {
-    return p->rows >= 1 && p->inputs >= 1 && p->inputs <= 131072 && p->outputs >= 1 && p->rows <= (1 << 30) && p->outputs <= (1 << 30);
 }
 
 }  // namespace seq
@@ -653,10 +621,11 @@ int tae_int8_linear(const tae_int8_args* p, void* stream) {
         }
         launch_quantize_dtype(QuantArgs{p->x, q, scale, p->x_row, qr, p->rows, p->inputs}, p->dtype, st);
         hipError_t e;
+        const Int8Form form = int8_form(p);
         switch (p->dtype) {
-            case TAE_DTYPE_F32: e = launch_int8<float>(a, st); break;
-            case TAE_DTYPE_F16: e = launch_int8<f16>(a, st); break;
-            default: e = launch_int8<bf16>(a, st); break;
+            case TAE_DTYPE_F32: e = launch_int8<float>(a, form, st); break;
+            case TAE_DTYPE_F16: e = launch_int8<f16>(a, form, st); break;
+            default: e = launch_int8<bf16>(a, form, st); break;
         }
         if (e != hipSuccess) return fail_msg(TAE_EHIP, hipGetErrorString(e));
         return (int)TAE_OK;

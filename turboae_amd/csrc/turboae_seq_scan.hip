@@ -17,8 +17,6 @@ struct ScanArgs {
     int64_t blocks;
 };
 
-constexpr int kScanThreads = 256;
-
 // Elements of a row as they were loaded, in whole registers and taken out only when they are used, so that a load stays in flight until
 // then.  V = 4: four adjacent ones, aligned to them; V = 1: four on any element, those of the row's end moved back inside it until `settle`;
 // V = 0: one, those behind the row repeat its last.
@@ -358,7 +356,7 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
 // wave's life where both should take 72).  So whichever has more positions left goes first.  Measured, bf16, 4096 positions x 4096 channels
 // x 16 states in 32 pieces: 90 us, ends pass 65 (four waves, no priorities: 90 and 68); fp32, 500 x 100 x 200 x 16: 48 (57).  More pieces,
 // so more waves, are no faster (48: 94 + 69, 64: 92 + 71), fewer are slower (16: 129 + 84).
-constexpr int kAhead = 8, kLaneWaves = 8;
+constexpr int kAhead = 8;
 
 template <class T, int N, bool ENDS>
 __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) {
@@ -641,8 +639,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int
 
 template <class T, int V, int EACH>
 static int launch_step(ScanArgs a, int batch, hipStream_t st) {
-    int lanes = 1;
-    while (lanes * V < a.n) lanes *= 2;
+    const int lanes = state_lanes(a.n, V);
     const int64_t groups = ceil_div(a.channels, kScanThreads / lanes);
     a.by_groups = Divisor(groups);
     a.blocks = groups * ceil_div(batch, EACH);
@@ -660,10 +657,9 @@ static int launch_step(ScanArgs a, int batch, hipStream_t st) {
     return TAE_OK;
 }
 
-// Four sequences for each workgroup, so that A is read once for them, as long as two workgroups for each CU remain.
 template <class T, int V>
 static int launch_steps(const ScanArgs& a, int batch, hipStream_t st) {
-    return batch >= 4 && (int64_t)a.channels * a.n / V * batch >= 4 * 512 * kScanThreads ? launch_step<T, V, 4>(a, batch, st) : launch_step<T, V, 1>(a, batch, st);
+    return step_sequences(batch, a.channels, a.n, V) == 4 ? launch_step<T, V, 4>(a, batch, st) : launch_step<T, V, 1>(a, batch, st);
 }
 
 // Few positions: as one position, P lanes for a channel with V adjacent states each, and all operands straight from memory, kNear positions
@@ -737,8 +733,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_short_kernel(ScanArgs q) {
 
 template <class T, int V>
 static int launch_short(ScanArgs a, int64_t batch, hipStream_t st) {
-    int lanes = 1;
-    while (lanes * V < a.n) lanes *= 2;
+    const int lanes = state_lanes(a.n, V);
     const int64_t groups = ceil_div(a.channels, kScanThreads / lanes);
     a.by_groups = Divisor(groups);
     a.blocks = groups * batch;
@@ -754,74 +749,6 @@ static int launch_short(ScanArgs a, int64_t batch, hipStream_t st) {
         default: hipLaunchKernelGGL((scan_short_kernel<T, 64, V>), grid, block, 0, st, a); break;
     }
     return TAE_OK;
-}
-
-// How a call is cut: lanes for a channel, each with per_lane states, and pieces along the positions.
-struct ScanPlan {
-    int lanes = 0, per_lane = 1, groups = 1, pieces = 1, piece_len = 0;       // lanes = 0: few positions, by scan_step_kernel or scan_short_kernel
-    size_t steps_bytes = 0, bytes = 0;
-};
-
-constexpr int kPieceUnit = 64;                   // pieces are whole tiles
-
-// The ways to share a channel's states (4, 8, 16, 32 or 64 with those filled up) among lanes: by scan_short_kernel (lanes = 0, four states
-// each), by scan_lane_kernel with one lane, else by selective_scan_kernel.  ns: what a wave takes for a position, with other waves on its
-// SIMD; alone: the number of waves whose time one by itself takes; start: us before a round of waves is under way, which up to 64
-// positions do not hide.  Measured over lengths from 2 to 8192 and 128 to 204800 channels of all sequences together, in bf16 with gate; what
-// follows from them is mostly within 16 % of the best of these ways and pieces, and within 9 us for few positions.
-//     us, pieces in (); batch x len x channels x states      1 lane      4 lanes     8 lanes     16 lanes
-//     1 x 4096 x 4096 x 16                                   146 (32)                136 (32)    163 (16)
-//     8 x 2048 x 1024 x 16                                   147 (16)                131 (8)     127 (1)
-//     1 x 2048 x 512 x 16                                     78 (32)                 24 (32)     26 (16)
-//     64 x 256 x 256 x 16                                     82 (4)                  31 (1)      37 (1)
-//     500 x 100 x 200 x 16                                    69 (1)                  71 (1)      91 (1)
-//     2 x 2048 x 2048 x 32                                                           128 (8)     122 (1)
-//     20 x 400 x 600 x 8                                      96 (4)      41 (1)      35 (1)
-//     40 x 569 x 416 x 4                                      79 (5)      62 (1)
-struct ScanForm {
-    int lanes, per_lane;
-    double ns, alone, start;
-};
-constexpr ScanForm kForms[] = {{0, 4, 232, 1.45, 1}, {0, 8, 180, 1.85, 1}, {0, 16, 152, 2.2, 1}, {0, 32, 130, 2.6, 1}, {0, 64, 138, 2.45, 1},
-                              {4, 1, 71, 1.15, 2}, {8, 1, 31, 1.7, 1}, {1, 16, 300, 1.8, 6}, {8, 2, 49, 1.45, 1}, {16, 1, 31, 1.5, 1.3}, {8, 4, 75, 1.5, 2},
-                              {16, 2, 45, 1.25, 2.5}, {16, 4, 96, 1.1, 4}};
-
-// Few channels leave SIMDs empty: then fewer states for each lane, or pieces along the positions, which cost a pass for their ends (0.6 of the
-// main one) and a launch that joins them (8 us).  The choice is the cheapest by these numbers and the waves that a SIMD (1024 of them) runs.
-static bool plan_scan(const tae_scan_args* p, ScanPlan* out) {
-    if (p->batch < 1 || p->len < 1 || p->channels < 1 || p->states < 1 || p->states > 64 || !dtype_ok(p->dtype)) return false;
-    if (p->len == 1) return true;
-    int padded = 4;
-    while (padded < p->states) padded *= 2;
-    double least = 0.0;
-    for (const ScanForm& f : kForms) {
-        const int share = f.lanes ? f.lanes : padded / 4;
-        if (f.per_lane * (f.lanes ? f.lanes : 1) != padded || (!f.lanes && p->len > 32)) continue;        // few positions: 32 at the most
-        const int64_t groups = ceil_div(p->channels, f.lanes == 1 ? 64 : kScanThreads / share);
-        for (int64_t pieces = 1; pieces <= (f.lanes ? 64 : 1); ++pieces) {
-            const int64_t piece_len = ceil_div(ceil_div(p->len, pieces), kPieceUnit) * kPieceUnit;
-            if (ceil_div(p->len, piece_len) < pieces) continue;
-            auto time = [&](int64_t n) {
-                const double cus = ceil_div(n * p->batch * groups, f.lanes == 1 ? kLaneWaves : 1) / 256.0;         // workgroups for each
-                const double all = f.lanes == 1 ? 2.0 * std::ceil(cus) : cus < 4.0 ? std::ceil(cus) : cus;          // waves for a SIMD of the fullest
-                return std::max(all, f.alone) * std::min<int64_t>(piece_len, p->len) * f.ns * 1e-3 + (p->len <= 64 ? f.start * std::max(all, 1.0) : 0.0);
-            };
-            const double cost = time(pieces) + (pieces > 1 ? 0.6 * time(pieces - 1) + 8.0 : 0.0);
-            if (least == 0.0 || cost < least) {
-                least = cost;
-                out->lanes = f.lanes;
-                out->per_lane = f.per_lane;
-                out->groups = (int)groups;
-                out->pieces = (int)pieces;
-                out->piece_len = (int)piece_len;
-            }
-        }
-    }
-    if (out->pieces > 1) {
-        out->steps_bytes = ((size_t)p->batch * out->pieces * p->channels * 4 + 255) / 256 * 256;
-        out->bytes = out->steps_bytes + (size_t)p->batch * (out->pieces + 1) * p->channels * p->states * 4;
-    }
-    return true;
 }
 
 static void launch_join(const ScanArgs& a, int64_t batch, hipStream_t st) {
