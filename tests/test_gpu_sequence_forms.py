@@ -67,3 +67,14 @@ def test_token_logprobs_in_its_larger_forms(gpu_device, dt, R, V, top, odd):
     logits = rnd(g, R, V, std=3.0, dtype=DT[dt])
     tokens = torch.randint(0, V, (R,), generator=g)
     check_logprobs(logits, tokens, top, gpu_device, wide(logits, gpu_device, 3, 2) if odd else None)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [33, 56, 57, 60, 61, 63, 64, 65, 504, 505, 508, 511, 512, 513])
+@pytest.mark.parametrize("left", [0, 1, 5])
+def test_token_logprobs_of_short_rows_that_start_anywhere(gpu_device, dt, V, left):
+    g = gen(V + left)
+    logits = rnd(g, 130, V, std=3.0, dtype=DT[dt])
+    tokens = torch.randint(0, V, (130,), generator=g)
+    for top in (0, 1, min(V, 32)):
+        check_logprobs(logits, tokens, top, gpu_device, wide(logits, gpu_device, left, 0))

@@ -1,11 +1,15 @@
 """Every form of the sequence operators' kernels is run by a test on the GPU: the lists of cases there, put through the library's own rules.  A
 change of a rule that leaves a form without a case fails here."""
+import ctypes
+
 import pytest
 
 from tests import _sequence_forms as F
 from tests import test_gpu_sequence as T
 from tests import test_gpu_sequence_edges as E
 from tests import test_gpu_sequence_forms as L
+from tests import test_sequence_cpu as C
+from turboae_amd import _lib
 
 
 @pytest.fixture(scope="module")
@@ -39,3 +43,12 @@ def test_every_form_of_token_logprobs_has_a_case(forms):
     cases = [(*c, aligned) for c in T.LOGP + L.LOGP_LARGE for aligned in (False, True)]
     found = {(lanes, elements, parts > 1) for lanes, elements, parts in forms.logprobs(cases)}
     assert found >= {(8, 8, False), (64, 8, False), (64, 32, False), (64, 32, True), (256, 32, False), (256, 32, True), (256, 64, False), (256, 64, True)}
+
+
+def test_short_rows_of_logits_are_one_part_wherever_they_start(forms):
+    """Rows that are read by single elements need no room for a granule that they start inside: one launch, no workspace."""
+    rows = [(dt, 1000, V, top, aligned) for dt in F.DTYPE for V in (33, 56, 57, 60, 61, 63, 64) for top in (0, 1, V // 2, 32) for aligned in (False, True)]
+    for case, (lanes, elements, parts) in zip(rows, forms.logprobs(rows)):
+        assert (lanes, elements, parts) == (8, 8, 1), case
+        a = C.build(_lib.TaeLogprobsArgs, dtype=F.DTYPE[case[0]], rows=case[1], vocab=case[2], top=case[3])
+        assert _lib.load().tae_token_logprobs_workspace(ctypes.byref(a)) == 0, case

@@ -148,26 +148,27 @@ struct LogprobsPlan {
     size_t stats_bytes = 0, bytes = 0;
 };
 
-// aligned_rows: every row starts on a 16-byte boundary (an unaligned part reaches into one granule more)
+// aligned_rows: every row starts on a 16-byte boundary.  An unaligned part that is read in granules of 16 bytes reaches into one more; rows of
+// up to 64 are read by single elements and do not.  (Nor are those of up to 512 with alternatives, but an unaligned one of 505 to 512 is no
+// worse off in granules: 20000 x 508 in bf16 with one alternative 16 us, by single elements 23; x 511 in fp32 with eight 23 and 20.)
 inline bool plan_logprobs(const tae_logprobs_args* p, bool aligned_rows, LogprobsPlan* s) {
     if (p->rows < 1 || p->vocab < 1 || p->vocab > (1 << 21) || p->top < 0 || p->top > 32 || p->top > p->vocab || !dtype_ok(p->dtype)) return false;
     const int V = 16 / (int)dtype_bytes(p->dtype);
     const int spare = aligned_rows ? 0 : V;
-    auto parts_of = [&](int lanes, int ept) {
+    auto parts_of = [&](int lanes, int ept, int most) {
         s->lanes = lanes;
         s->ept = ept;
-        const int most = lanes * ept - spare;
         s->parts = (int)ceil_div(p->vocab, most);
         s->part_len = (int)std::min<int64_t>(most, ceil_div(ceil_div(p->vocab, s->parts), 8) * 8);
         s->parts = (int)ceil_div(p->vocab, s->part_len);
     };
     // the fewest lanes that hold a row; long rows in parts, smaller ones where few rows would leave SIMDs empty
     const int64_t elements = (int64_t)p->rows * p->vocab;
-    if (p->vocab <= 64) parts_of(8, 8);
-    else if (p->vocab <= 512 - spare) parts_of(64, 8);      // with alternatives single elements: all lanes have some, and so a close bound of them
-    else if (p->vocab <= 2048 - spare || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32);
-    else if (p->vocab <= 8192 - spare || (elements < (int64_t)1024 * 8192 && p->vocab <= (1 << 20))) parts_of(256, 32);
-    else parts_of(256, 64);
+    if (p->vocab <= 64) parts_of(8, 8, 64);
+    else if (p->vocab <= 512 - spare) parts_of(64, 8, 512 - spare);     // with alternatives single elements: all lanes have some, and so a close bound of them
+    else if (p->vocab <= 2048 - spare || (elements < (int64_t)2048 * 2048 && p->vocab <= (1 << 18))) parts_of(64, 32, 2048 - spare);
+    else if (p->vocab <= 8192 - spare || (elements < (int64_t)1024 * 8192 && p->vocab <= (1 << 20))) parts_of(256, 32, 8192 - spare);
+    else parts_of(256, 64, 16384 - spare);
     if (s->parts > 1) {
         s->stats_bytes = (size_t)p->rows * s->parts * 16;
         s->bytes = s->stats_bytes + (size_t)p->rows * s->parts * p->top * 8;
