@@ -38,6 +38,7 @@ int main() {
 """
 
 DTYPE = {"f32": 0, "f16": 1, "bf16": 2}
+TILES = ((4, 1), (8, 1), (16, 1), (8, 2), (16, 2), (8, 4), (16, 4))          # lanes for a channel, states of each
 INT8_FORMS = ["rows", "few16", "few32", "few64", "tiles128", "tiles128_two", "tiles256"]
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import _sequence_oracle as O
-from tests.test_gpu_sequence import DT, check_logprobs, gen, inside, int8_case, rnd, rows16, run_scan, scan_case, wide
+from tests.test_gpu_sequence import DT, INF, check_logprobs, gen, inside, int8_case, rnd, rows16, run_scan, scan_case, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,33 @@ def test_token_logprobs_of_short_rows_that_start_anywhere(gpu_device, dt, V, lef
     tokens = torch.randint(0, V, (130,), generator=g)
     for top in (0, 1, min(V, 32)):
         check_logprobs(logits, tokens, top, gpu_device, wide(logits, gpu_device, left, 0))
+
+
+# states that fill the lanes of every form, and states that do not
+INFINITE = [("bf16", 1, 15, 3, 9), ("f32", 1, 15, 4, 9), ("f16", 1, 300, 3, 9), ("bf16", 1, 300, 4, 9), ("f32", 1, 15, 3, 17), ("bf16", 1, 15, 4, 17), ("f32", 1, 300, 3, 28), ("f16", 1, 300, 4, 17),
+            ("bf16", 1, 15, 3, 33), ("f32", 1, 15, 4, 33), ("bf16", 1, 200, 7, 33), ("f16", 1, 200, 4, 33), ("f32", 1, 7, 3, 1), ("bf16", 1, 7, 4, 2), ("bf16", 1, 300, 3, 3), ("f32", 1, 300, 4, 1),
+            ("f16", 1, 2, 3, 5), ("f32", 1, 2, 4, 5), ("bf16", 1, 300, 3, 7), ("f32", 1, 300, 4, 5), ("bf16", 1, 2, 3, 11), ("f32", 1, 2, 4, 9), ("f16", 1, 500, 1562, 9), ("bf16", 1, 421, 1788, 9),
+            ("f32", 1, 7, 3, 28), ("bf16", 1, 7, 4, 17), ("f32", 1, 421, 1871, 17), ("bf16", 1, 421, 1852, 17), ("bf16", 9, 7, 14288, 9), ("f32", 1, 2048, 4096, 9),
+            ("f32", 1, 2, 13260, 9), ("bf16", 1, 2, 3, 17), ("f16", 1, 2, 4, 3), ("f32", 1, 2, 4, 33), ("bf16", 1, 2, 8704, 5), ("f32", 1, 2, 9452, 12), ("bf16", 1, 2, 3, 20),
+            ("f32", 3, 1, 33, 5), ("bf16", 3, 1, 70, 12), ("f32", 257, 1, 2051, 12),
+            ("bf16", 1, 15, 3, 16), ("f32", 1, 15, 4, 16), ("f16", 1, 15, 3, 32), ("bf16", 1, 15, 4, 32), ("f32", 1, 15, 3, 64), ("f16", 1, 15, 4, 64), ("bf16", 1, 7, 3, 4), ("f32", 1, 7, 4, 4), ("bf16", 1, 7, 3, 8),
+            ("f16", 1, 7, 4, 8), ("f32", 1, 7, 3, 16), ("bf16", 1, 7, 4, 16), ("bf16", 1, 7, 3, 32), ("f32", 1, 7, 4, 32), ("bf16", 6, 7, 2713, 4), ("f32", 1, 7, 3, 64), ("bf16", 9, 15, 13176, 16)]
+
+
+@pytest.mark.parametrize("dt,B,L,E,N", INFINITE)
+def test_infinities_come_out_as_the_formula_has_them(gpu_device, dt, B, L, E, N):
+    """An infinite input, an infinite step and an infinite incoming state, each in a channel of its own, with everything positive: infinite
+    from there on, no NaN, and other channels as they are.  Steps are small, so that no decay underflows to 0 (0 times infinity is NaN)."""
+    c = scan_case(B + L + E + N, dt, B, L, E, N, True, True, None)
+    for name in ("x", "B", "C", "D", "z", "state"):
+        c[name] = c[name].abs() + 0.0625
+    c["dt"] = c["dt"].clamp(-1.0, 1.0)
+    c["dt_bias"] = torch.full((E,), -7.0)
+    c["x"][0, L // 2, 0] = INF
+    c["dt"][0, L // 2, 1] = INF
+    c["state"][B - 1, E - 1, N - 1] = INF
+    y, h, by, bh = O.scan(**c)
+    assert not bool(torch.isnan(y).any()) and bool(torch.isinf(y[0, L // 2:, :2]).all()) and bool(torch.isinf(y[B - 1, :, E - 1]).all())
+    got, state = run_scan(c, gpu_device, strided=False)
+    inside(got, y, by, "y")
+    inside(state, h, bh, "state")

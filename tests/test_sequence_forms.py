@@ -22,10 +22,19 @@ def forms(tmp_path_factory):
 def test_every_form_of_the_scan_has_a_case(forms):
     cases = [(("bf16", "f32", "f16")[sum(c) % 3], *c) for c in E.FORMS] + [c[:5] for c in T.SCAN] + L.SCANS
     want = {("lane", full, cut) for full in (False, True) for cut in (False, True)}
-    want |= {("tile", lanes, per_lane, cut, V) for lanes, per_lane in ((4, 1), (8, 1), (16, 1), (8, 2), (16, 2), (8, 4), (16, 4)) for cut in (False, True) for V in (1, 4)}
+    want |= {("tile", lanes, per_lane, cut, V) for lanes, per_lane in F.TILES for cut in (False, True) for V in (1, 4)}
     want |= {("short", 4, 1 << i) for i in range(5)} | {("short", 1, 1 << i) for i in range(7)}
     want |= {("step", 4, 1 << i, each) for i in range(5) for each in (1, 4)} | {("step", 1, 1 << i, each) for i in range(7) for each in (1, 4)}
     assert set(forms.scan(cases)) == want
+
+
+def test_every_form_of_the_scan_meets_infinities(forms):
+    """With states that fill its lanes and with states that do not; pieces only matter to the latter."""
+    found = {form[:-1] + ("cut" if form[-1] else "whole",) if form[0] == "lane" else form + (c[4] == form[1] * form[2],) if form[0] == "tile" else form[:3] for form, c in
+             zip(forms.scan(L.INFINITE), L.INFINITE)}
+    tiles = {("tile", *split, cut, V, False) for split in F.TILES for cut in (False, True) for V in (1, 4)} | {("tile", *split, False, V, True) for split in F.TILES for V in (1, 4)}
+    assert found >= tiles | {("lane", False, "whole"), ("lane", False, "cut"), ("lane", True, "whole")}
+    assert found >= {("short", 4, 1 << i) for i in (2, 3, 4)} | {("short", 1, 1 << i) for i in range(2, 7)} | {("step", 4, 4), ("step", 1, 8)}
 
 
 def test_every_form_of_int8_linear_has_a_case(forms):

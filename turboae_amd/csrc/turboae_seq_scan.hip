@@ -84,13 +84,14 @@ __device__ __forceinline__ int reduced_position(int lane) {
 // piece in tiles of TT: steps d and d x (once for each channel and position), B and C go through LDS as rows over the positions, so that a
 // lane reads four positions with one 16-byte load; two buffers, one barrier for each tile; the next tile's loads are in flight meanwhile.
 // ENDS: only the state behind a piece, started from zero (the first piece: from `state`), and the sum of its steps, whose exponential
-// carries a state across the piece.  V: 4 where rows allow loads of four channels, else 1.
+// carries a state across the piece.  V: 4 where rows allow loads of four channels, else 1.  FILLED: some states only fill lanes up.  Their B and C
+// are 0, but an infinite step or input makes NaN of them, so they are left out of the sums by choice.
 //
 // Bound by issuing: with 16 states in P = 8, S = 2 a wave takes 45 ns for a position of its 8 channels, of which 26 are the states' 12 issue
 // slots (two products, exp of two slots, two fused) and the rest sums over lanes, LDS, softplus and gate.  More lanes for a channel spread few
 // channels over the chip and share softplus and gate, for longer sums over lanes; what each split takes stands at kForms.  Measured, bf16:
 // 2048 x 512 channels x 16 states 10 us and 9 for the ends, 8 x 512 x 256 x 64 34 and 17, 256 x 2048 x 16 in one piece 15.
-template <class T, int S, int P, int TT, int V, bool ENDS>
+template <class T, int S, int P, int TT, int V, bool ENDS, bool FILLED>
 __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q) {
     constexpr int CW = kScanThreads / P, N = S * P, DS = TT + 4;
     constexpr int R = TT * CW / 4 / kScanThreads, RB = (TT * N + kScanThreads - 1) / kScanThreads;      // groups of four, elements for each thread
@@ -255,13 +256,27 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
                 }
                 float out[4];
 #pragma unroll
-                for (int s = 0; s < S; ++s)
+                for (int s = 0; s < S; ++s) {
+                    float at[4];                 // the state behind each position
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float g = __builtin_amdgcn_exp2f(d4.v[i] * a2[s]);
-                        h[s] = __builtin_fmaf(g, h[s], x4.v[i] * b4[s].v[i]);
-                        if constexpr (!ENDS) out[i] = s == 0 ? h[s] * c4[s].v[i] : __builtin_fmaf(h[s], c4[s].v[i], out[i]);
+                        at[i] = h[s] = __builtin_fmaf(g, h[s], x4.v[i] * b4[s].v[i]);
+                        if (!ENDS && (!FILLED || S == 1 || 2 * s < S)) out[i] = s == 0 ? at[i] * c4[s].v[i] : __builtin_fmaf(at[i], c4[s].v[i], out[i]);
                     }
+                    if constexpr (!ENDS && FILLED) {
+                        if constexpr (S == 1) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) out[i] = p < q.n ? out[i] : 0.0f;
+                        } else if (2 * s >= S) {         // more than half of all states are in use
+                            if (s * P + p < q.n) {
+                                asm volatile("");            // a branch: with four choices 50 x 410 x 480 x 12 takes 57 us, so 54
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) out[i] = __builtin_fmaf(at[i], c4[s].v[i], out[i]);
+                            }
+                        }
+                    }
+                }
                 if constexpr (ENDS) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum += d4.v[i];
@@ -355,10 +370,10 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
 // left alone the older of two gets most of the issue slots and the younger runs by itself at the end, at half the rate (61 and 83 us of a
 // wave's life where both should take 72).  So whichever has more positions left goes first.  Measured, bf16, 4096 positions x 4096 channels
 // x 16 states in 32 pieces: 90 us, ends pass 65 (four waves, no priorities: 90 and 68); fp32, 500 x 100 x 200 x 16: 48 (57).  More pieces,
-// so more waves, are no faster (48: 94 + 69, 64: 92 + 71), fewer are slower (16: 129 + 84).
+// so more waves, are no faster (48: 94 + 69, 64: 92 + 71), fewer are slower (16: 129 + 84).  FILLED: as above.
 constexpr int kAhead = 8;
 
-template <class T, int N, bool ENDS>
+template <class T, int N, bool ENDS, bool FILLED>
 __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) {
     constexpr int W = ENDS ? N : 2 * N, RB = (kAhead * W + 63) / 64;       // values of B (and C) for each position; loads of each lane
     __shared__ alignas(16) float lds[kLaneWaves][2][kAhead * W];
@@ -492,7 +507,14 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
             for (int k = 0; k < G; ++k) h[k0 + k] = __builtin_fmaf(g[k], h[k0 + k], u[k]);
             if constexpr (!ENDS) {
 #pragma unroll
-                for (int k = 0; k < G; ++k) out[i] = __builtin_fmaf(h[k0 + k], cv[at & 1][k], out[i]);
+                for (int k = 0; k < (FILLED && k0 ? G / 2 : G); ++k)
+                    if (!FILLED || k0 + k <= N / 2 || k0 + k < q.n) out[i] = __builtin_fmaf(h[k0 + k], cv[at & 1][k], out[i]);      // more than half are in use
+                if (FILLED && k0 && k0 + G / 2 < q.n) {
+                    asm volatile("");            // a branch for all lanes: up to 12 states pay three choices and save four products
+#pragma unroll
+                    for (int k = G / 2; k < G; ++k)
+                        if (k0 + k < q.n) out[i] = __builtin_fmaf(h[k0 + k], cv[at & 1][k], out[i]);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -717,7 +739,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_short_kernel(ScanArgs q) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 h.v[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a.v[j]), h.v[j], dx * now.b[i][j]);
-                out = __builtin_fmaf(h.v[j], mine ? now.c[i][j] : 0.0f, out);
+                if (mine) out = __builtin_fmaf(h.v[j], now.c[i][j], out);
             }
             out = __builtin_fmaf(dcoef, now.x[i][0], lanes_sum<P>(out));
             if (q.gate) out *= silu(now.z[i][0]);
@@ -759,10 +781,11 @@ static void launch_join(const ScanArgs& a, int64_t batch, hipStream_t st) {
 template <class T, int S, int P, int TT, int V>
 static void launch_scan_as(const ScanArgs& a, int64_t batch, hipStream_t st) {
     if (a.pieces > 1) {
-        hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, true>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
+        hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, true, false>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
         launch_join(a, batch, st);
     }
-    hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, false>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
+    if (a.n == S * P) hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, false, false>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
+    else hipLaunchKernelGGL((selective_scan_kernel<T, S, P, TT, V, false, true>), grid_of(a.blocks), dim3(kScanThreads), 0, st, a);
 }
 
 template <class T, int S, int P, int TT>
@@ -775,10 +798,11 @@ template <class T, int N>
 static int launch_lane(const ScanArgs& a, int64_t batch, hipStream_t st) {
     const dim3 grid = grid_of(ceil_div(a.blocks, kLaneWaves)), block(kLaneWaves * 64);
     if (a.pieces > 1) {
-        hipLaunchKernelGGL((scan_lane_kernel<T, N, true>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((scan_lane_kernel<T, N, true, false>), grid, block, 0, st, a);
         launch_join(a, batch, st);
     }
-    hipLaunchKernelGGL((scan_lane_kernel<T, N, false>), grid, block, 0, st, a);
+    if (a.n == N) hipLaunchKernelGGL((scan_lane_kernel<T, N, false, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((scan_lane_kernel<T, N, false, true>), grid, block, 0, st, a);
     return TAE_OK;
 }
 
