@@ -108,3 +108,21 @@ def test_infinities_come_out_as_the_formula_has_them(gpu_device, dt, B, L, E, N)
     got, state = run_scan(c, gpu_device, strided=False)
     inside(got, y, by, "y")
     inside(state, h, bh, "state")
+
+
+@pytest.mark.parametrize("dt,B,L,E,N", [("f32", 2, 1, 40, 4), ("bf16", 33, 1, 16328, 1), ("f16", 3, 2, 9, 3), ("bf16", 2, 2, 4395, 12), ("f32", 2, 15, 6, 16), ("bf16", 2, 300, 8, 9), ("f16", 1, 300, 5, 4),
+                                        ("f32", 9, 15, 13176, 16), ("f32", 1, 2048, 4096, 9)])
+def test_an_absent_direct_term_adds_nothing_to_an_infinity(gpu_device, dt, B, L, E, N):
+    """Without D an infinite x comes out of the states alone; a D of zeros makes NaN of it, as the formula does."""
+    c = scan_case(B + L + E + N, dt, B, L, E, N, False, False, None)
+    for name in ("x", "B", "C"):
+        c[name] = c[name].abs() + 0.0625
+    c["dt"], c["dt_bias"] = c["dt"].clamp(-1.0, 1.0), torch.full((E,), -7.0)
+    c["x"][0, L // 2, 0] = INF
+    for D in (None, torch.zeros(E)):
+        c["D"] = D
+        y, h, by, bh = O.scan(**c)
+        assert bool(torch.isinf(y[0, L // 2, 0])) == (D is None)
+        got, state = run_scan(c, gpu_device, strided=False)
+        inside(got, y, by, "y")
+        inside(state, h, bh, "state")

@@ -329,7 +329,8 @@ __global__ __launch_bounds__(kScanThreads) void selective_scan_kernel(ScanArgs q
                 for (int i = 0; i < 4; ++i) {
                     float v = 0.0f;
                     if (at < stop) {
-                        v = __builtin_fmaf(dcoef[i], now.x[j][i], sy[buf][(cq + i) * DS + tt]);
+                        v = sy[buf][(cq + i) * DS + tt];
+                        if (q.d) v = __builtin_fmaf(dcoef[i], now.x[j][i], v);         // not 0 times an infinite x
                         if (q.gate) v *= silu(now.z[j][i]);
                     }
                     o.v[i] = (T)v;
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
         for (int i = 0; i < kAhead; ++i) {
             const float xv = now.x[i][0];
             dx[i] = d[i] * xv;
-            out[i] = dcoef * xv;
+            out[i] = q.d ? dcoef * xv : 0.0f;    // not 0 times an infinite x
             if constexpr (ENDS) sum += i < count ? d[i] : 0.0f;
         }
         // G states at a time: their products, exps, products and fused adds each as G instructions in a row, so that none waits for the one in
@@ -649,7 +650,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs q, int
                 if (mine) out = __builtin_fmaf(h[i].v[j], cm[i][j], out);
             }
             out = lanes_sum<P>(out);
-            out = __builtin_fmaf(dcoef, x[i][0], out);
+            if (q.d) out = __builtin_fmaf(dcoef, x[i][0], out);
             if (q.gate) out *= silu(z[i][0]);
         }
         if (b < batch && e < E) {
@@ -741,7 +742,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_short_kernel(ScanArgs q) {
                 h.v[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a.v[j]), h.v[j], dx * now.b[i][j]);
                 if (mine) out = __builtin_fmaf(h.v[j], now.c[i][j], out);
             }
-            out = __builtin_fmaf(dcoef, now.x[i][0], lanes_sum<P>(out));
+            out = lanes_sum<P>(out);
+            if (q.d) out = __builtin_fmaf(dcoef, now.x[i][0], out);
             if (q.gate) out *= silu(now.z[i][0]);
             if (p == 0 && e < E) y[(int64_t)(t0 + i) * E] = (T)out;
         }
