@@ -126,3 +126,18 @@ def test_an_absent_direct_term_adds_nothing_to_an_infinity(gpu_device, dt, B, L,
         got, state = run_scan(c, gpu_device, strided=False)
         inside(got, y, by, "y")
         inside(state, h, bh, "state")
+
+
+@pytest.mark.parametrize("dt,B,L,E,N", [("f32", 1, 300, 4, 9), ("bf16", 1, 700, 64, 16), ("f32", 1, 2048, 4096, 16), ("f32", 1, 300, 4, 64)])
+def test_infinite_states_outlast_a_piece_of_the_positions(gpu_device, dt, B, L, E, N):
+    """A position's factor is e^-5, that of the 64 and more positions of a piece 0 in 32 bits: an infinite state stays one all the same."""
+    c = scan_case(B + L + E + N, dt, B, L, E, N, False, True, None)
+    for name in ("x", "B", "C", "state"):
+        c[name] = c[name].abs() + 0.0625
+    c.update(A=torch.full((E, N), -5.0), dt=torch.ones_like(c["dt"]), dt_bias=None, softplus=False)
+    c["state"][0, E // 2, N - 1] = INF
+    y, h, by, bh = O.scan(**c)
+    assert bool(torch.isinf(y[0, :, E // 2]).all()) and int(torch.isinf(h).sum()) == 1
+    got, state = run_scan(c, gpu_device, strided=False)
+    inside(got, y, by, "y")
+    inside(state, h, bh, "state")

@@ -593,8 +593,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs q, int
         for (int j = 0; j < A; ++j) {
             if (j0 + j < q.pieces) {
                 slot[(j0 + j) * step] = h;
-                // by its root twice: the whole factor may be infinite (a growing state) where its product is not; a state of 0 stays one
-                const float root = __builtin_amdgcn_exp2f(0.5f * sum[j] * a2);
+                // by its root twice: the whole factor may be infinite (a growing state) where its product is not; a state of 0 stays one.  A root
+                // of finite steps is 2^-126 at least: 2^-252 of a state is nothing, but an infinite one, which no position makes finite, stays one
+                const float exponent = 0.5f * sum[j] * a2;
+                const float root = __builtin_amdgcn_exp2f(exponent < -126.0f && exponent > -__builtin_inff() ? -126.0f : exponent);
                 h = h == 0.0f ? part[j] : __builtin_fmaf(root, root * h, part[j]);
             }
         }
