@@ -362,8 +362,10 @@ TAE_API int tae_causal_conv(const tae_conv_args* args, void* stream);
 
 /* Selective state-space scan.  Per channel e and state n, with d = softplus(dt + dt_bias) (or dt + dt_bias with softplus = 0):
  *     h[t] = exp(d[t] A[e,n]) h[t-1] + d[t] B[t,n] x[t,e],   y[t,e] = (sum_n C[t,n] h[t] + D[e] x[t,e]) * z[t,e] sigmoid(z[t,e])
- * h starts at `state` (NULL: zeros) and its last value goes to state_out (which may be state itself; required).  Long inputs with few
- * channels are cut along t and joined again in fixed order: results do not depend on timing.  len = 1 is the single-token step. */
+ * h starts at `state` (NULL: zeros) and its last value goes to state_out (which may be state itself; required).  Without d, z or dt_bias their
+ * terms are left out, not taken with zeros.  Long inputs with few channels are cut along t and joined again in fixed order: results do not
+ * depend on timing.  An infinite input or state makes what the formula makes of it, decays that 32 bits hold as 0 apart (0 * infinity).
+ * len = 1 is the single-token step. */
 typedef struct tae_scan_args {
     int32_t struct_size;          /* = sizeof(tae_scan_args) */
     int32_t dtype;                /* x, dt, B, C, z, y */
@@ -393,8 +395,7 @@ TAE_API int tae_selective_scan(const tae_scan_args* args, void* stream);
  *     r = residual + alpha * scale * gate_act(gate) * p          (block NULL: r = residual)
  *     normed = norm(r) * pre_weight + pre_bias                   (of r before its rounding)
  * norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps), mean = 0 with center = 0.  residual_out may be residual itself (same strides).
- * Squares are summed in fp32: norm is 0 for a row whose
- * sum of squares is not finite there. */
+ * Squares are summed in fp32: norm is 0 for finite values whose sum of squares is not finite there. */
 typedef struct tae_norm_args {
     int32_t struct_size;          /* = sizeof(tae_norm_args) */
     int32_t dtype;                /* block, gate, normed */

@@ -141,3 +141,20 @@ def test_infinite_states_outlast_a_piece_of_the_positions(gpu_device, dt, B, L, 
     got, state = run_scan(c, gpu_device, strided=False)
     inside(got, y, by, "y")
     inside(state, h, bh, "state")
+
+
+def test_leading_dimensions_that_do_not_fold_are_copied(gpu_device):
+    """Rows that no single distance leads through, and last elements that are apart in three dimensions; in two they are refused."""
+    from turboae_amd import sequence
+    g, dev = gen(6), gpu_device
+    x, w, s, b = int8_case(g, torch.bfloat16, 24, 48, 20)
+    rows, q, s, b = x.view(4, 6, 48).to(dev), rows16(w, dev), s.to(dev), b.to(dev)
+    logits, tokens = rnd(g, 4, 6, 300).to(dev), torch.randint(0, 300, (4, 6), generator=g).to(dev)
+    for pick in (lambda v: v[:, 1:5], lambda v: v.transpose(0, 1), lambda v: v.mT.contiguous().mT):
+        assert torch.equal(sequence.int8_linear(pick(rows), q, s, b), sequence.int8_linear(pick(rows).contiguous(), q, s, b))
+        t = pick(tokens[..., None])[..., 0].contiguous()
+        for a, e in zip(sequence.token_logprobs(pick(logits), t, top=4), sequence.token_logprobs(pick(logits).contiguous(), t, top=4)):
+            assert torch.equal(a, e)
+    for call in (lambda: sequence.int8_linear(rows[0].t().contiguous().t(), q, s, b), lambda: sequence.token_logprobs(logits[0].t().contiguous().t(), tokens[0])):
+        with pytest.raises(ValueError, match="adjacent"):
+            call()

@@ -16,7 +16,9 @@ Activations are float32, float16 or bfloat16, (batch, len, channels) with adjace
 without a copy; parameters and states named float32 are float32.  Sums, norms, softmax statistics and states are kept in 32 bits or more
 and each result is rounded once.  ``lengths`` (int32, one for each sequence) marks padding: positions at or behind it are not read, their
 outputs are zero, and the state is the one after the last position in front of them.  Sizes, rows of all leading dimensions together among
-them, are below 2^31.
+them, are below 2^31.  ``int8_linear`` and ``token_logprobs`` take any number of leading dimensions: rows that one distance leads through are
+taken as they lie; other inputs of three and more dimensions are copied first, as ``reshape`` does it, and a matrix whose last elements are
+apart is refused.
 """
 from __future__ import annotations
 
