@@ -28,17 +28,21 @@ constexpr int kPieceUnit = 64;                   // pieces are whole tiles
 // The ways to share a channel's states (4, 8, 16, 32 or 64 with those filled up) among lanes: by scan_short_kernel (lanes = 0, four states
 // each), by scan_lane_kernel with one lane, else by selective_scan_kernel.  ns: what a wave takes for a position, with other waves on its
 // SIMD; alone: the number of waves whose time one by itself takes; start: us before a round of waves is under way, which up to 64
-// positions do not hide.  Measured over lengths from 2 to 8192 and 128 to 204800 channels of all sequences together, in bf16 with gate; what
-// follows from them is mostly within 16 % of the best of these ways and pieces, and within 9 us for few positions.
-//     us, pieces in (); batch x len x channels x states      1 lane      4 lanes     8 lanes     16 lanes
-//     1 x 4096 x 4096 x 16                                   146 (32)                136 (32)    163 (16)
-//     8 x 2048 x 1024 x 16                                   147 (16)                131 (8)     127 (1)
-//     1 x 2048 x 512 x 16                                     78 (32)                 24 (32)     26 (16)
-//     64 x 256 x 256 x 16                                     82 (4)                  31 (1)      37 (1)
-//     500 x 100 x 200 x 16                                    69 (1)                  71 (1)      91 (1)
-//     2 x 2048 x 2048 x 32                                                           128 (8)     122 (1)
-//     20 x 400 x 600 x 8                                      96 (4)      41 (1)      35 (1)
-//     40 x 569 x 416 x 4                                      79 (5)      62 (1)
+// positions do not hide.  Fitted to lengths from 2 to 8192 and 128 to 204800 channels of all sequences together, in bf16 with gate.  What is
+// taken is not always the best: up to 15 % behind it in the list, which gives whole calls at the best number of pieces.
+//     us, pieces in (); batch x len x channels x states      1 lane      4 lanes     8 lanes     16 lanes    taken
+//     1 x 4096 x 4096 x 16                                   149 (32)                144 (16)    169 (5)     1 lane (32)
+//     8 x 2048 x 1024 x 16                                   147 (16)                136 (8)     128 (1)     16 lanes (1)
+//     1 x 2048 x 512 x 16                                     78 (32)                 24 (32)     27 (16)    8 lanes (32)
+//     64 x 256 x 256 x 16                                     85 (4)                  30 (1)      38 (1)     8 lanes (1)
+//     500 x 100 x 200 x 16                                    68 (1)                  65 (1)      86 (1)     1 lane (1)
+//     500 x 100 x 200 x 16, fp32, no gate                     61 (1)                  63 (1)      81 (1)     1 lane (1)
+//     2 x 2048 x 2048 x 32                                                           127 (8)     125 (1)     16 lanes (1)
+//     20 x 400 x 600 x 8                                                              34 (1)                 8 lanes (1)
+//     40 x 569 x 416 x 4                                                  62 (1)                             4 lanes (9), 68
+//     8 x 512 x 256 x 64                                                                          51 (1)     16 lanes (4), 59
+//     78 x 3961 x 16 x 8                                                              71 (16)                8 lanes (31), 71
+// Sequences are counted with all of their positions, whatever `lengths` holds.
 struct ScanForm {
     int lanes, per_lane;
     double ns, alone, start;
