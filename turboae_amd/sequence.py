@@ -43,7 +43,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 class _Call:
     """The checks that every tensor of a call goes through, against the first of them; a call of a single token costs little more."""
 
-    __slots__ = ("name", "device", "dtype", "grad", "tangents", "new")
+    __slots__ = ("name", "device", "dtype", "grad", "new")
 
     def __init__(self, name: str, first: torch.Tensor):
         if not isinstance(first, torch.Tensor) or not first.is_cuda:
@@ -51,12 +51,11 @@ class _Call:
         if first.dtype not in _DTYPE:
             raise ValueError(f"{name}: float32, float16 or bfloat16 wanted, got {first.dtype}")
         self.name, self.device, self.dtype, self.grad, self.new = name, first.device, first.dtype, torch.is_grad_enabled(), first.new_empty
-        self.tangents = getattr(forward_ad, "_current_level", 0) >= 0              # inside a dual_level, the only place for tangents
+        if getattr(forward_ad, "_current_level", 0) >= 0:                          # inside a dual_level, the only place for tangents
+            self.__class__ = _CallAmongTangents
 
-    def sizes(self, *sizes: int) -> None:
-        """The library's sizes have 32 bits, and ctypes would cut larger ones to them."""
-        if max(sizes) > 0x7FFFFFFF:
-            raise ValueError(f"{self.name}: sizes must be below 2^31, got {sizes}")
+    def too_large(self, *sizes: int) -> None:
+        raise ValueError(f"{self.name}: sizes must be below 2^31, got {sizes}")
 
     def tensor(self, t: Optional[torch.Tensor], what: str, shape: Tuple[int, ...], dtype: torch.dtype, dense: bool = False) -> Optional[int]:
         """Address of a tensor after its checks (None for None): shape, type, device, adjacent last elements; dense: contiguous."""
@@ -71,8 +70,6 @@ class _Call:
                 raise ValueError(f"{self.name}: adjacent elements of {what}'s last dimension must be adjacent in memory")
         if self.grad and t.requires_grad:
             raise ValueError(f"{self.name}: {what} requires a gradient, but this path is inference only (call it under torch.no_grad())")
-        if self.tangents and forward_ad.unpack_dual(t).tangent is not None:      # torch.no_grad() does not turn tangents off
-            raise ValueError(f"{self.name}: {what} has a forward-mode tangent, but this path is inference only (call it with unpack_dual's primal)")
         return t.data_ptr()
 
     def out(self, t: Optional[torch.Tensor], what: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
@@ -91,8 +88,7 @@ class _Call:
         args.workspace, args.workspace_bytes = w.data_ptr(), n
         return w
 
-    def run(self, entry, *args, writes: Optional[torch.Tensor] = None) -> None:
-        """`writes`: a tensor of the caller that the call changes; autograd sees it as after any operation in place."""
+    def run(self, entry, *args) -> None:
         index = self.device.index
         if torch.cuda.current_device() == index:
             rc = entry(*args, _raw_stream(index))
@@ -101,15 +97,29 @@ class _Call:
                 rc = entry(*args, _raw_stream(index))
         if rc:
             _lib.check(rc)
-        if writes is not None:
-            increment_version(writes)
+
+
+class _CallAmongTangents(_Call):
+    """The same where tensors may have forward-mode tangents, which torch.no_grad() does not turn off."""
+
+    __slots__ = ()
+
+    def tensor(self, t, what, shape, dtype, dense=False):
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{self.name}: {what} has a forward-mode tangent, but this path is inference only (call it with unpack_dual's primal)")
+        return super().tensor(t, what, shape, dtype, dense)
+
+
+_MOST = 0x7FFFFFFF                               # the library's sizes have 32 bits, and ctypes would cut larger ones to them
 
 
 def _sequence(c: _Call, what: str, t: torch.Tensor) -> Tuple[int, int, int]:
     if t.dim() != 3 or t.numel() == 0:
         raise ValueError(f"{c.name}: {what} must have shape (batch, len, channels), none of them 0, got {tuple(t.shape)}")
-    c.sizes(*t.shape)
-    return t.shape
+    shape = t.shape
+    if max(shape) > _MOST:
+        c.too_large(*shape)
+    return shape
 
 
 def _strides(t: Optional[torch.Tensor]) -> Tuple[int, int]:
@@ -156,7 +166,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                             c.tensor(x, "x", (B, L, E), c.dtype), c.tensor(weight, "weight", (E, K), f32, True), c.tensor(bias, "bias", (E,), f32, True),
                             c.tensor(state, "state", (B, K - 1, E), c.dtype, True) if K > 1 else None,
                             c.tensor(lengths, "lengths", (B,), torch.int32, True), y.data_ptr(), state_out.data_ptr() if K > 1 else None)
-    c.run(_lib.load().tae_causal_conv, ctypes.byref(args), writes=given)
+    c.run(_lib.load().tae_causal_conv, ctypes.byref(args))
+    if given is not None:                        # autograd sees it as after any operation in place
+        increment_version(given)
     return y, state_out
 
 
@@ -190,7 +202,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
                             y.data_ptr(), state_out.data_ptr(), None, 0)
     lib = _lib.load()
     w = c.workspace(args, lib.tae_selective_scan_workspace)  # noqa: F841
-    c.run(lib.tae_selective_scan, ctypes.byref(args), writes=given)
+    c.run(lib.tae_selective_scan, ctypes.byref(args))
+    if given is not None:                        # autograd sees it as after any operation in place
+        increment_version(given)
     return y, state_out
 
 
@@ -245,7 +259,9 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
                             *_strides(residual), *_strides(block), *ga, *_strides(out), c.tensor(residual, "residual", (B, L, D), residual.dtype),
                             c.tensor(block, "block", (B, L, D), c.dtype), None if gate is None else gate.data_ptr(), *vectors,
                             out.data_ptr() if write else None, None if normed is None else normed.data_ptr())
-    c.run(_lib.load().tae_norm_residual, ctypes.byref(args), writes=residual_out if write else None)
+    c.run(_lib.load().tae_norm_residual, ctypes.byref(args))
+    if write and residual_out is not None:
+        increment_version(residual_out)
     return out, normed
 
 
@@ -257,7 +273,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if x.dim() != 2 or 0 in x.shape:
         raise ValueError(f"quantize_int8: x must have shape (rows, columns), none of them 0, got {tuple(x.shape)}")
     R, K = x.shape
-    c.sizes(R, K)
+    if max(R, K) > _MOST:
+        c.too_large(R, K)
     address = c.tensor(x, "x", (R, K), c.dtype)
     step = -(-K // 64) * 64
     q = c.new((R, step), dtype=torch.int8)
@@ -275,7 +292,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise ValueError(f"int8_linear: x (..., inputs) and weight (outputs, inputs) wanted, none of them 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
     N, K = weight.shape
     M = x.numel() // x.shape[-1]
-    c.sizes(M, N)
+    if M > _MOST or N > _MOST:
+        c.too_large(M, N)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if K > 131072:
         raise ValueError(f"int8_linear: at most 131072 inputs, got {K}")
@@ -310,7 +328,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not 0 <= top <= min(32, V) or V > 1 << 21:
         raise ValueError(f"token_logprobs: top must be in 0..32 and at most vocab, vocab at most 2^21, got {top} of {V}")
     R = logits.numel() // V
-    c.sizes(R)
+    if R > _MOST:
+        c.too_large(R)
     flat = logits if logits.dim() == 2 else logits.reshape(-1, V)
     shape = tuple(tokens.shape)
     logp = c.new(shape, dtype=torch.float32)
