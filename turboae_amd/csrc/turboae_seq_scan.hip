@@ -568,7 +568,7 @@ __global__ __launch_bounds__(kLaneWaves * 64) void scan_lane_kernel(ScanArgs q) 
 
 // The state in front of every piece from those behind them: slot k of `states` holds what piece k - 1 left (slot 0 nothing yet), and gets
 // what piece k starts from.  The first piece has started from `state`.  One lane for a state; bound by waiting for its loads, 8 pieces at a
-// time (6.9 us for 32 pieces of 65536 states; 16 or 32 at a time the same).
+// time (7.1 us for 32 pieces of 65536 states; 16 or 32 at a time the same).
 __global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs q, int64_t count) {
     const int64_t i = block_index() * kScanThreads + threadIdx.x;
     if (i >= count) return;
