@@ -84,7 +84,7 @@ def test_token_logprobs_of_short_rows_that_start_anywhere(gpu_device, dt, V, lef
 INFINITE = [("bf16", 1, 15, 3, 9), ("f32", 1, 15, 4, 9), ("f16", 1, 300, 3, 9), ("bf16", 1, 300, 4, 9), ("f32", 1, 15, 3, 17), ("bf16", 1, 15, 4, 17), ("f32", 1, 300, 3, 28), ("f16", 1, 300, 4, 17),
             ("bf16", 1, 15, 3, 33), ("f32", 1, 15, 4, 33), ("bf16", 1, 200, 7, 33), ("f16", 1, 200, 4, 33), ("f32", 1, 7, 3, 1), ("bf16", 1, 7, 4, 2), ("bf16", 1, 300, 3, 3), ("f32", 1, 300, 4, 1),
             ("f16", 1, 2, 3, 5), ("f32", 1, 2, 4, 5), ("bf16", 1, 300, 3, 7), ("f32", 1, 300, 4, 5), ("bf16", 1, 2, 3, 11), ("f32", 1, 2, 4, 9), ("f16", 1, 500, 1562, 9), ("bf16", 1, 421, 1788, 9),
-            ("f32", 1, 7, 3, 28), ("bf16", 1, 7, 4, 17), ("f32", 1, 421, 1871, 17), ("bf16", 1, 421, 1852, 17), ("bf16", 9, 7, 14288, 9), ("f32", 1, 2048, 4096, 9),
+            ("f32", 1, 7, 3, 28), ("bf16", 1, 7, 4, 17), ("f32", 1, 421, 1871, 17), ("bf16", 1, 421, 1852, 17), ("bf16", 9, 7, 14288, 9), ("f32", 9, 15, 13176, 14), ("f32", 1, 2048, 4096, 9), ("bf16", 1, 2048, 4096, 13),
             ("f32", 1, 2, 13260, 9), ("bf16", 1, 2, 3, 17), ("f16", 1, 2, 4, 3), ("f32", 1, 2, 4, 33), ("bf16", 1, 2, 8704, 5), ("f32", 1, 2, 9452, 12), ("bf16", 1, 2, 3, 20),
             ("f32", 3, 1, 33, 5), ("bf16", 3, 1, 70, 12), ("f32", 257, 1, 2051, 12),
             ("bf16", 1, 15, 3, 16), ("f32", 1, 15, 4, 16), ("f16", 1, 15, 3, 32), ("bf16", 1, 15, 4, 32), ("f32", 1, 15, 3, 64), ("f16", 1, 15, 4, 64), ("bf16", 1, 7, 3, 4), ("f32", 1, 7, 4, 4), ("bf16", 1, 7, 3, 8),

@@ -34,6 +34,8 @@ def test_every_form_of_the_scan_meets_infinities(forms):
              zip(forms.scan(L.INFINITE), L.INFINITE)}
     tiles = {("tile", *split, cut, V, False) for split in F.TILES for cut in (False, True) for V in (1, 4)} | {("tile", *split, False, V, True) for split in F.TILES for V in (1, 4)}
     assert found >= tiles | {("lane", False, "whole"), ("lane", False, "cut"), ("lane", True, "whole")}
+    halves = {c[4] > 12 for form, c in zip(forms.scan(L.INFINITE), L.INFINITE) if form[0] == "lane" and c[4] < 16}
+    assert halves == {False, True}                                # with and without states in the last quarter of a lane
     assert found >= {("short", 4, 1 << i) for i in (2, 3, 4)} | {("short", 1, 1 << i) for i in range(2, 7)} | {("step", 4, 4), ("step", 1, 8)}
 
 
